@@ -95,6 +95,49 @@ class AttnArgs(C.Structure):
                 ("counters_len", C.c_uint32), ("err", C.c_void_p), ("pdl", C.c_int)]
 
 
+class KvPlanArgs(C.Structure):
+    """b2_kv_plan_args (include/b2_kernels.h): page tables, positions and slots from lengths."""
+    _fields_ = [("batch", C.c_uint32), ("max_rows", C.c_uint32), ("page_tokens", C.c_uint32),
+                ("pages_per_seq", C.c_uint32), ("pool_pages", C.c_uint32), ("ctx_len", C.c_void_p),
+                ("new_len", C.c_void_p), ("tree", C.c_void_p), ("mapped", C.c_void_p), ("free_pages", C.c_void_p),
+                ("free_count", C.c_void_p), ("page_table", C.c_void_p), ("mapped_out", C.c_void_p),
+                ("free_out", C.c_void_p), ("row_start", C.c_void_p), ("row_item", C.c_void_p),
+                ("row_pos", C.c_void_p), ("row_slot", C.c_void_p), ("err", C.c_void_p), ("pdl", C.c_int)]
+
+
+class RowsAppendArgs(C.Structure):
+    """b2_rows_append_args (include/b2_kernels.h): RoPE and K/V into cache slots."""
+    _fields_ = [("m", C.c_uint32), ("y", C.c_void_p), ("y_stride", C.c_uint32), ("q_rows", C.c_uint32),
+                ("q", C.c_void_p), ("q_stride", C.c_uint32), ("rope_freq", C.c_void_p), ("positions", C.c_void_p),
+                ("slots", C.c_void_p), ("n_rows", C.c_void_p), ("kv", KVLayout), ("pool_pages", C.c_uint32),
+                ("err", C.c_void_p), ("pdl", C.c_int)]
+
+
+class AttnRowsArgs(C.Structure):
+    """b2_attn_rows_args (include/b2_kernels.h): trees or chunks of rows over the paged cache."""
+    _fields_ = [("batch", C.c_uint32), ("n_heads", C.c_uint32), ("n_kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32), ("max_rows", C.c_uint32), ("rows", C.c_uint32), ("q", C.c_void_p),
+                ("q_stride", C.c_uint32), ("kv", KVLayout), ("pool_pages", C.c_uint32), ("row_start", C.c_void_p),
+                ("ctx_len", C.c_void_p), ("tree", C.c_void_p), ("max_ctx", C.c_uint32), ("ctx", C.c_void_p),
+                ("ctx_stride", C.c_uint32), ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t),
+                ("err", C.c_void_p), ("pdl", C.c_int)]
+
+
+class TreeAcceptArgs(C.Structure):
+    """b2_tree_accept_args (include/b2_kernels.h): greedy verification of drafted trees."""
+    _fields_ = [("batch", C.c_uint32), ("max_rows", C.c_uint32), ("rows", C.c_uint32), ("row_start", C.c_void_p),
+                ("tokens", C.c_void_p), ("tree", C.c_void_p), ("argmax", C.c_void_p), ("ctx_len", C.c_void_p),
+                ("path", C.c_void_p), ("count", C.c_void_p), ("next", C.c_void_p), ("ctx_out", C.c_void_p),
+                ("err", C.c_void_p), ("pdl", C.c_int)]
+
+
+class KvCompactArgs(C.Structure):
+    """b2_kv_compact_args (include/b2_kernels.h): taken rows' K/V moved together in every layer."""
+    _fields_ = [("n_layers", C.c_uint32), ("layers", C.POINTER(KVLayout)), ("pool_pages", C.c_uint32),
+                ("batch", C.c_uint32), ("ctx_len", C.c_void_p), ("path", C.c_void_p), ("count", C.c_void_p),
+                ("err", C.c_void_p), ("pdl", C.c_int)]
+
+
 class ModelTensor(C.Structure):
     _fields_ = [("name", C.c_char * 64), ("dtype", C.c_uint32), ("ndims", C.c_uint32),
                 ("shape", C.c_uint64 * 4), ("offset", C.c_uint64), ("nbytes", C.c_uint64),
@@ -264,6 +307,12 @@ _SIGS = {
     "b2_gemm": (C.c_int, [C.POINTER(GemmArgs), _P]),
     "b2_attn_scratch_bytes": (_SZ, [C.POINTER(AttnArgs)]),
     "b2_attn": (C.c_int, [C.POINTER(AttnArgs), _P]),
+    "b2_kv_plan": (C.c_int, [C.POINTER(KvPlanArgs), _P]),
+    "b2_rows_append": (C.c_int, [C.POINTER(RowsAppendArgs), _P]),
+    "b2_attn_rows_scratch_bytes": (_SZ, [C.POINTER(AttnRowsArgs)]),
+    "b2_attn_rows": (C.c_int, [C.POINTER(AttnRowsArgs), _P]),
+    "b2_tree_accept": (C.c_int, [C.POINTER(TreeAcceptArgs), _P]),
+    "b2_kv_compact": (C.c_int, [C.POINTER(KvCompactArgs), _P]),
     "b2_rmsnorm": (C.c_int, [_P, _P, _P, _U32, _F, _P]),
     "b2_softmax": (C.c_int, [_P, _U32, _P]),
     "b2_rope": (C.c_int, [_P, _U32, _U32, _F, _P]),

@@ -27,6 +27,8 @@ extern "C" {
 #define B2_ERR_POSITION    0x4  /* position outside the KV capacity */
 #define B2_ERR_NAN_LOGITS  0x8  /* NaN in logits (greedy sampler rejects) */
 #define B2_ERR_TOKEN       0x10 /* token id outside the vocabulary */
+#define B2_ERR_CAPACITY    0x20 /* rows or pages beyond what the caller provided */
+#define B2_ERR_TREE        0x40 /* an ancestor mask that no tree has */
 
 /* ---- quantised weights in device layout ---------------------------------- */
 /*
@@ -407,6 +409,163 @@ typedef struct b2_rows_args {
     int pdl;
 } b2_rows_args;
 int b2_rows_epilogue(const b2_rows_args *a, void *stream);
+
+/* ---- several new rows per sequence: drafted trees and prompt chunks -------- */
+/*
+ * A step that adds a varying number of rows to each of several sequences: the
+ * nodes of a drafted token tree to be verified, or a chunk of prompt tokens.
+ * Item b has row_start[b+1] - row_start[b] consecutive rows (0 allowed) after
+ * ctx_len[b] cached tokens; row i of the item (its local index) keeps its K/V
+ * at cache place ctx_len[b] + i. `tree` gives each row the set of the item's
+ * rows it attends besides the cached tokens, bit j = local row j, itself
+ * included: for a tree, row 0 is the token just decoded (the root), parents
+ * come before children, and the mask is the row's ancestors and itself, at
+ * most B2_MAX_TREE rows per item. NULL is the causal chain: row i attends rows
+ * 0..i, and an item may have any number of rows.
+ *
+ *   b2_kv_plan -> per layer (b2_gemm, b2_rows_append, b2_attn_rows, ...) ->
+ *   logits and argmax keys of every row -> b2_tree_accept -> b2_kv_compact
+ *
+ * Every array is device memory (except where a comment says host); outputs
+ * must not overlap inputs. Rows at and after row_start[batch] are left as they
+ * were. No counterpart in the reference, which decodes one token at a time.
+ */
+#define B2_MAX_TREE 64         /* rows of an item with ancestor masks */
+#define B2_MAX_PLAN_BATCH 4096 /* sequences of one b2_kv_plan */
+
+/* Row starts, positions, cache slots and page tables of a step from the
+ * sequences' lengths, pages taken from a stack of free ones: sequence b then
+ * holds max(mapped[b], ceil((ctx_len[b] + new_len[b]) / page_tokens)) pages;
+ * its missing ones are the top of the stack downwards, sequences and their
+ * pages in order. A row's position is ctx_len[b] plus its depth in the tree
+ * (its mask's bits less one), or plus its local index without a tree; its slot
+ * is page * page_tokens + offset in the pool. A step that does not fit
+ * (max_rows, the free pages: B2_ERR_CAPACITY; a sequence past its table row or
+ * with cached tokens on no page, a negative length, more than B2_MAX_TREE rows
+ * with a tree: B2_ERR_POSITION) changes no page table and gives every sequence
+ * zero rows (row_start all 0, mapped_out and free_out as their inputs). A page
+ * id outside [0, pool_pages) raises B2_ERR_POSITION and its rows get slot -1. */
+typedef struct b2_kv_plan_args {
+    uint32_t batch;              /* 1..B2_MAX_PLAN_BATCH */
+    uint32_t max_rows;           /* length of the row arrays */
+    uint32_t page_tokens, pages_per_seq, pool_pages;
+    const int32_t *ctx_len;      /* [batch] */
+    const int32_t *new_len;      /* [batch] */
+    const uint64_t *tree;        /* [max_rows] or NULL */
+    const int32_t *mapped;       /* [batch] pages in use in each table row */
+    const int32_t *free_pages;   /* [>= free_count] */
+    const int32_t *free_count;   /* one value */
+    int32_t *page_table;         /* [batch][pages_per_seq], updated in place */
+    int32_t *mapped_out;         /* [batch] */
+    int32_t *free_out;           /* one value */
+    int32_t *row_start;          /* [batch + 1] */
+    int32_t *row_item, *row_pos, *row_slot; /* [max_rows] */
+    int32_t *err;
+    int pdl;
+} b2_kv_plan_args;
+int b2_kv_plan(const b2_kv_plan_args *a, void *stream);
+
+/* B2_EPI_QKV of b2_rows_epilogue with each row's position and cache slot given
+ * apart: rows y of q | k | v, RoPE of q (to `q`) and k at positions[n], k and v
+ * stored in slot slots[n] of the pools (kv.page_table is not used). The same
+ * roundings as b2_rows_epilogue. slots[n] < 0 stores no K/V; a slot past the
+ * pool or a negative position raises B2_ERR_POSITION and the row's K/V (and,
+ * for the position, its q) are left as they were. */
+typedef struct b2_rows_append_args {
+    uint32_t m;                  /* rows of the arrays */
+    const float *y;              /* [m][y_stride], 16-byte aligned, stride a multiple of 4 */
+    uint32_t y_stride;           /* >= q_rows + 2 * n_kv_heads * head_dim */
+    uint32_t q_rows;             /* a multiple of head_dim */
+    float *q;                    /* [m][q_stride] */
+    uint32_t q_stride;
+    const float *rope_freq;      /* [head_dim/2], NULL: no RoPE */
+    const int32_t *positions;    /* [m]; not read without RoPE */
+    const int32_t *slots;        /* [m], no two live rows the same */
+    const int32_t *n_rows;       /* rows in use (e.g. row_start + batch), NULL: all m */
+    b2_kv_layout kv;
+    uint32_t pool_pages;
+    int32_t *err;
+    int pdl;
+} b2_rows_append_args;
+int b2_rows_append(const b2_rows_append_args *a, void *stream);
+
+/* Attention of the new rows over the paged cache, their own K/V included (so
+ * after b2_rows_append): softmax(q k / sqrt(head_dim)) v over the cached tokens
+ * and the rows that `tree` (or the causal chain) lets a row see. Row n of q and
+ * ctx holds all heads. A row that sees nothing (no cached token, mask 0) gets
+ * zeros. Cache places past an item's rows are not read. A NaN or infinity in
+ * the K or V of a place makes the rows that see it NaN (in the query heads of
+ * that KV head) and raises B2_ERR_NONFINITE; rows that do not see it are as if
+ * it were finite. The same holds for a NaN or infinity in a row of q. An item
+ * whose lengths do not fit (max_rows, rows, max_ctx, B2_MAX_TREE) or a
+ * negative page id (or, with pool_pages given, one past the pool) raises
+ * B2_ERR_POSITION; such an item's rows are left as they were, such a page's
+ * places are not seen. Products are kept to about 2^-22 (see the kernel); the
+ * result does not depend on timing. */
+typedef struct b2_attn_rows_args {
+    uint32_t batch, n_heads, n_kv_heads, head_dim; /* head_dim a multiple of 16, at most 128 */
+    uint32_t max_rows;           /* most rows of one item (sizes the grid) */
+    uint32_t rows;               /* rows of q and ctx */
+    const float *q;              /* [rows][q_stride] (RoPE applied), 16-byte aligned */
+    uint32_t q_stride;           /* a multiple of 4 */
+    b2_kv_layout kv;             /* page_table [batch][pages_per_seq] */
+    uint32_t pool_pages;         /* 0: page ids are not checked against the pool's size */
+    const int32_t *row_start;    /* [batch + 1] */
+    const int32_t *ctx_len;      /* [batch] */
+    const uint64_t *tree;        /* [rows] or NULL: causal */
+    uint32_t max_ctx;            /* most places (cached and new) of one item */
+    float *ctx;                  /* [rows][ctx_stride] */
+    uint32_t ctx_stride;
+    void *scratch;               /* b2_attn_rows_scratch_bytes, any contents, 16-byte aligned */
+    size_t scratch_bytes;
+    int32_t *err;
+    int pdl;
+} b2_attn_rows_args;
+size_t b2_attn_rows_scratch_bytes(const b2_attn_rows_args *a); /* 0: none needed, or invalid arguments */
+int b2_attn_rows(const b2_attn_rows_args *a, void *stream);
+
+/* Greedy verification of drafted trees: from the root on, a row's argmax token
+ * picks the child that carries it (the lowest local index among equals), until
+ * no child does. path[b] = the local rows taken (ascending, row 0 first, -1
+ * behind the last), count[b] how many, next[b] the last one's argmax token,
+ * ctx_out[b] = ctx_len[b] + count[b]. An item without rows: count 0, next
+ * 0xFFFFFFFF. A mask that no tree has (without its own bit or row 0, bits at or
+ * past the row) raises B2_ERR_TREE and its row is not taken; a row count that
+ * does not fit raises B2_ERR_POSITION (count 0). tree NULL: a chain. */
+typedef struct b2_tree_accept_args {
+    uint32_t batch;
+    uint32_t max_rows;           /* most rows of one item, at most B2_MAX_TREE */
+    uint32_t rows;
+    const int32_t *row_start;    /* [batch + 1] */
+    const uint32_t *tokens;      /* [rows] the rows' tokens */
+    const uint64_t *tree;        /* [rows] or NULL */
+    const unsigned long long *argmax; /* [rows] keys of the rows' logits (b2_rows_epilogue) */
+    const int32_t *ctx_len;      /* [batch] */
+    int32_t *path;               /* [batch][B2_MAX_TREE] */
+    int32_t *count;              /* [batch] */
+    uint32_t *next;              /* [batch] */
+    int32_t *ctx_out;            /* [batch] */
+    int32_t *err;
+    int pdl;
+} b2_tree_accept_args;
+int b2_tree_accept(const b2_tree_accept_args *a, void *stream);
+
+/* The K/V of the taken rows moved together in every layer: cache place
+ * ctx_len[b] + path[b][i] to ctx_len[b] + i for i < count[b] (path[b][i] >= i,
+ * ascending; others, and places outside the table row, raise B2_ERR_POSITION
+ * and are not moved). ctx_len is the length before the step. */
+typedef struct b2_kv_compact_args {
+    uint32_t n_layers;
+    const b2_kv_layout *layers;  /* host [n_layers], one geometry */
+    uint32_t pool_pages;         /* 0: page ids are not checked against the pool's size */
+    uint32_t batch;
+    const int32_t *ctx_len;      /* [batch] */
+    const int32_t *path;         /* [batch][B2_MAX_TREE] */
+    const int32_t *count;        /* [batch] */
+    int32_t *err;
+    int pdl;
+} b2_kv_compact_args;
+int b2_kv_compact(const b2_kv_compact_args *a, void *stream);
 
 /* ---- element ops (backend vtable on device buffers) ---------------------- */
 int b2_rmsnorm(float *dst, const float *src, const float *w, uint32_t n, float eps, void *stream);
