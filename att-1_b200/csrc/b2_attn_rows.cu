@@ -9,21 +9,20 @@
 // Work split. The rows of an item times the query heads of one KV head are the
 // rows r = token * group + head of a matrix; CTA (split, KV head and block of
 // 128 such rows, item) takes a contiguous range of the places in tiles of 64, so
-// K and V are read once per 128 rows. 13 warps (at most four per scheduler: 128
-// registers a thread):
-//   warps 8..11   load K and V (f32) straight into registers, eight keys ahead of
-//                 the eight being converted, and store them as matrix operands;
-//                 the tiles to come are asked into L2, so that a register load's
-//                 round trip is L2's and not HBM's;
-//   warp 12       one thread issues the tcgen05 MMAs: S = Q K^T of tile j + 1
-//                 before O = P V of tile j, accumulators in tensor memory, two
-//                 buffers each;
+// K and V are read once per 128 rows. 16 warps (128 registers a thread):
+//   warp 15       streams K and V (f32) into a ring of tiles with bulk copies, a
+//                 run of places on one page each;
+//   warps 8..13   convert: units of eight places' K or V from the ring into matrix
+//                 operands;
+//   warp 14       one thread issues the tcgen05 MMAs: S = Q K^T of tile j + 1
+//                 before O = P V of tile j; Q, P, S and O live in tensor memory
+//                 (O in two buffers), only K and V are read from shared memory;
 //   warps 0..7    two per 32 rows: a thread holds one row and 32 of a tile's 64
-//                 keys: scores from tensor memory, the row's running maximum
-//                 (joined with the other half's through shared memory), P as
-//                 matrix operand; then one row and half of the dimensions of O,
-//                 summed in registers over the tiles, so a growing maximum
-//                 rescales registers, not tensor memory.
+//                 places: its scores from tensor memory, the row's running maximum
+//                 (over all 64, so the two need not talk), P back into tensor
+//                 memory; and half of the dimensions of the row's O, summed in
+//                 registers over the tiles: a growing maximum rescales registers,
+//                 not tensor memory, and no sum runs through more than 12 MMAs.
 // Splits write (maximum, sum, weighted values) per row; a second kernel joins
 // them in split order. No counters or atomics: results do not depend on timing.
 //
@@ -31,18 +30,21 @@
 // exact): hi = f16(x 2^e), lo = f16(x 2^e - hi), and a product is
 // hi hi + lo hi + hi lo with f32 accumulation; what is dropped is below 2^-22.
 // f16 rather than bf16 pairs (2^-16) because the scale takes care of the range:
-// a row of q, eight keys' K and eight keys' V have a power of two each that
-// brings their largest magnitude to [2^8, 2^9), so an element 2^-17 of the
-// largest still keeps 16 bits. K's scale goes into the scores, V's into P
-// relative to the tile's largest, and the tile's into its O when it is summed.
-// The softmax statistics and the weighted sums are f32.
+// a row of q, eight places' K and eight places' V have a power of two each that
+// brings their largest magnitude to [2^8, 2^12), so an element 2^-17 of the
+// largest still keeps 16 bits. (The exponents are multiples of four, so that
+// neighbours mostly share one and the factors below drop out.) K's scale goes
+// into the scores, V's into P relative to the tile's largest, and the tile's
+// into its O when it is summed. The softmax statistics and the weighted sums are
+// f32.
 //
-// Operands are K-major without swizzle as in b2_gemm.cu: 8-row x 16-byte core
-// matrices, row groups 128 bytes apart, 8-column chunks R * 16 bytes apart. K's
-// hi and lo rows are one operand of 128 rows (one MMA of N = 128 gives
-// q_hi k_hi and q_hi k_lo, a second of N = 64 adds q_lo k_hi); V is transposed
-// on the way from registers to shared memory (a lane holds eight keys of a
-// dimension: one 16-byte store).
+// Operands in shared memory are K-major without swizzle as in b2_gemm.cu: 8-row
+// x 16-byte core matrices, row groups 128 bytes apart, 8-column chunks R * 16
+// bytes apart. V is transposed on its way through the registers (a lane holds
+// eight places of a dimension: one 16-byte store). Operand A of every MMA comes
+// from tensor memory, two f16 to a column: 128 rows of A would cost as many
+// shared-memory cycles per MMA as B does, and shared memory is what a tile of 64
+// places uses most (copies in 64 KB, conversion 64 + 64 KB, MMAs 96 KB).
 #include "b2_common.cuh"
 #include "b2_umma.cuh"
 
@@ -53,32 +55,31 @@ namespace b2 {
 constexpr uint32_t kRowsM = 128;        // (token, query head) rows of a CTA
 constexpr uint32_t kRowsKeys = 64;      // places of a tile
 constexpr int kRowsSoftWarps = 8;
-constexpr int kRowsConvWarps = 4;
-constexpr int kRowsThreads = 32 * (kRowsSoftWarps + kRowsConvWarps + 1);
-constexpr uint32_t kRowsMeta = 8;       // ring of per-tile K scales: more than the tiles between converting and softmax
-constexpr uint32_t kRowsAhead = 3;      // tiles ahead of the conversion whose K and V are asked into L2
+constexpr int kRowsConvWarps = 6;
+constexpr uint32_t kRowsMmaWarp = kRowsSoftWarps + kRowsConvWarps, kRowsCopyWarp = kRowsMmaWarp + 1;
+constexpr int kRowsThreads = 32 * (kRowsSoftWarps + kRowsConvWarps + 2);
+constexpr uint32_t kRowsMeta = 8;       // ring of per-tile scales: more than the tiles between converting and softmax
 constexpr uint32_t kRowsMaxSplits = 64;
-constexpr int kRowsTop = 8;             // operands are scaled to [2^kRowsTop, 2^(kRowsTop + 1))
+constexpr int kRowsTop = 8;             // operands are scaled to [2^kRowsTop, 2^(kRowsTop + 4))
 constexpr float kRowsP = 12.0f;         // P is scaled by 2^12
 
 template <int HD>
 struct RowsSmem {
-    static constexpr uint32_t stages = HD == 128 ? 2 : 4;
-    static constexpr uint32_t q_half = kRowsM * HD * 2;            // hi or lo
-    static constexpr uint32_t k_stage = 2 * kRowsKeys * HD * 2;    // hi and lo rows of one operand
-    static constexpr uint32_t v_half = kRowsKeys * HD * 2;
-    static constexpr uint32_t p_half = kRowsM * kRowsKeys * 2;
-    static constexpr uint32_t off_q = 0;
-    static constexpr uint32_t off_k = off_q + 2 * q_half;
-    static constexpr uint32_t off_v = off_k + stages * k_stage;
-    static constexpr uint32_t off_p = off_v + stages * 2 * v_half;
-    static constexpr uint32_t off_x = off_p + 2 * p_half;          // [2][2][128] f32: the halves' maxima
-    static constexpr uint32_t off_ks = off_x + 2 * 2 * kRowsM * 4;  // [kRowsMeta][8] f32: 1 / K scale of eight keys
-    static constexpr uint32_t off_km = off_ks + kRowsMeta * 8 * 4;  // [kRowsMeta][8] u32: keys that are NaN | hidden << 8
-    static constexpr uint32_t off_ve = off_km + kRowsMeta * 8 * 4;  // [4][8] int: exponent of eight keys' V
-    static constexpr uint32_t off_vm = off_ve + 4 * 8 * 4;          // [4][8] u32: keys whose V is NaN
-    static constexpr uint32_t off_bar = off_vm + 4 * 8 * 4;
-    static constexpr uint32_t bytes = off_bar + 8 * (4 * stages + 4 + 1 + 4 + 2 + 4) + 16;
+    static constexpr uint32_t k_stages = HD == 128 ? 1 : 2, v_stages = 2;
+    static constexpr uint32_t slots = HD == 128 ? 4 : 6;           // ring of f32 tiles, K and V in turn
+    static constexpr uint32_t slot = kRowsKeys * HD * 4;
+    static constexpr uint32_t half = kRowsKeys * HD * 2;           // hi or lo of an operand
+    static constexpr uint32_t off_k = 0;
+    static constexpr uint32_t off_v = off_k + k_stages * 2 * half;
+    static constexpr uint32_t off_r = off_v + v_stages * 2 * half;
+    static constexpr uint32_t off_x = off_r + slots * slot;         // [2][128] f32: the halves' sums
+    static constexpr uint32_t off_ks = off_x + 2 * kRowsM * 4;      // [kRowsMeta][8] f32: 1 / K scale of a unit
+    static constexpr uint32_t off_km = off_ks + kRowsMeta * 8 * 4;  // [kRowsMeta][8] u32: places that are NaN | hidden << 8
+    static constexpr uint32_t off_ve = off_km + kRowsMeta * 8 * 4;  // [2][8] int: exponent of a unit's V
+    static constexpr uint32_t off_vm = off_ve + 2 * 8 * 4;          // [2][8] u32: places whose V is NaN
+    static constexpr uint32_t off_rh = off_vm + 2 * 8 * 4;          // [slots] u64: places whose page is bad
+    static constexpr uint32_t off_bar = off_rh + 8 * slots;
+    static constexpr uint32_t bytes = off_bar + 8 * (2 * slots + 2 * k_stages + 2 * v_stages + 13) + 16;
 };
 static_assert(RowsSmem<128>::bytes <= 227 * 1024 && RowsSmem<64>::bytes <= 227 * 1024, "shared memory");
 
@@ -125,9 +126,9 @@ __device__ __forceinline__ float ex2(float x)
 
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126..127
 
-// Unbiased exponent of the largest magnitude (its bits), floored so that the
-// scale 2^(kRowsTop - e) and its inverse stay normal.
-__device__ __forceinline__ int top_exp(uint32_t amax_bits) { return max((int)(amax_bits >> 23) - 127, -100); }
+// Exponent of the largest magnitude (its bits), down to a multiple of four and
+// floored so that the scale 2^(kRowsTop - e) and its inverse stay normal.
+__device__ __forceinline__ int top_exp(uint32_t amax_bits) { return max(((int)(amax_bits >> 23) - 127) & ~3, -100); }
 
 // f16 hi and lo words of two values.
 __device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32_t &lo)
@@ -150,6 +151,15 @@ __device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[1
         : "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // All lanes wait; false for the whole warp if any gave up.
@@ -158,24 +168,26 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase, int32_t
     return __all_sync(0xffffffffu, mbar_wait_bounded(bar, phase & 1u, err));
 }
 
-template <int HD>
+template <int HD, bool EXACT>
 __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsParams p)
 {
     using S = RowsSmem<HD>;
-    constexpr uint32_t NST = S::stages;
+    constexpr uint32_t KST = S::k_stages, VST = S::v_stages, NR = S::slots;
     extern __shared__ __align__(1024) uint8_t smem[];
     const b2_attn_rows_args &a = p.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t split = blockIdx.x, kvh = blockIdx.y / p.blocks, blk = blockIdx.y % p.blocks, item = blockIdx.z;
-    const uint32_t hd = a.head_dim;
-    float *xmax = reinterpret_cast<float *>(smem + S::off_x);
+    const uint32_t hd = EXACT ? HD : a.head_dim;  // EXACT: head_dim == HD
+    float *xsum = reinterpret_cast<float *>(smem + S::off_x);
     float *kscale = reinterpret_cast<float *>(smem + S::off_ks);
     uint32_t *kmark = reinterpret_cast<uint32_t *>(smem + S::off_km);
     int *vexp = reinterpret_cast<int *>(smem + S::off_ve);
     uint32_t *vmark = reinterpret_cast<uint32_t *>(smem + S::off_vm);
-    uint64_t *k_full = reinterpret_cast<uint64_t *>(smem + S::off_bar), *k_empty = k_full + NST, *v_full = k_empty + NST,
-             *v_empty = v_full + NST, *s_full = v_empty + NST, *s_empty = s_full + 2, *p_full = s_empty + 2,
-             *o_full = p_full + 1, *o_empty = o_full + 2, *q_full = o_empty + 2, *done = q_full + 1, *xbar = done + 1;
+    uint64_t *rhide = reinterpret_cast<uint64_t *>(smem + S::off_rh);
+    uint64_t *r_full = reinterpret_cast<uint64_t *>(smem + S::off_bar), *r_empty = r_full + NR, *k_full = r_empty + NR,
+             *k_empty = k_full + KST, *v_full = k_empty + KST, *v_empty = v_full + VST, *s_full = v_empty + VST,
+             *s_empty = s_full + 1, *p_full = s_empty + 1, *o_full = p_full + 1, *o_empty = o_full + 2, *q_full = o_empty + 2,
+             *done = q_full + 1, *xbar = done + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(xbar + 4);
 
     pdl_wait();
@@ -196,86 +208,97 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
     const uint32_t nsoft = 2 * ((live + 31) / 32);  // softmax warps with rows: two per quarter of the rows
 
     if (threadIdx.x == 0) {
-        for (uint32_t i = 0; i < NST; ++i) {
-            mbar_init(&k_full[i], kRowsConvWarps);
+        for (uint32_t i = 0; i < NR; ++i) {
+            mbar_init(&r_full[i], 1);
+            mbar_init(&r_empty[i], kRowsKeys / 8);
+        }
+        for (uint32_t i = 0; i < KST; ++i) {
+            mbar_init(&k_full[i], kRowsKeys / 8);
             mbar_init(&k_empty[i], 1);
-            mbar_init(&v_full[i], kRowsConvWarps);
+        }
+        for (uint32_t i = 0; i < VST; ++i) {
+            mbar_init(&v_full[i], kRowsKeys / 8);
             mbar_init(&v_empty[i], 1);
         }
+        mbar_init(s_full, 1);
+        mbar_init(s_empty, nsoft);
+        mbar_init(p_full, nsoft);
         for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&s_empty[i], nsoft);
             mbar_init(&o_full[i], 1);
             mbar_init(&o_empty[i], nsoft);
         }
-        mbar_init(p_full, nsoft);
         mbar_init(q_full, nsoft);
         mbar_init(done, 1);
         for (uint32_t i = 0; i < 4; ++i) mbar_init(&xbar[i], 2);
         fence_mbar_init();
     }
-    if (warp == kRowsSoftWarps + kRowsConvWarps) tmem_alloc(tmem_slot, 512);
+    if (warp == kRowsMmaWarp) tmem_alloc(tmem_slot, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;  // S: columns 0..255 (two buffers of hi | lo keys), O: 256 + buffer * HD
+    const uint32_t tmem = *tmem_slot;
+    // columns: S 64 | P hi 32, lo 32 | Q hi HD / 2, lo HD / 2 | O from 256, two buffers of HD
+    const uint32_t tm_s = tmem, tm_p = tmem + 64, tm_q = tmem + 128, tm_o = tmem + 256;
 
-    if (warp >= (uint32_t)kRowsSoftWarps && warp < (uint32_t)(kRowsSoftWarps + kRowsConvWarps)) {
-        // ---- K and V into operands: keys 16 cw .. 16 cw + 15 of every tile, eight at a time ----
-        const uint32_t cw = warp - kRowsSoftWarps, key = lane & 7, ch = lane >> 3;
+    if (warp == kRowsCopyWarp) {
+        // ---- K and V tiles into the ring: lane l looks after places l and l + 32 ----
         const int32_t *table = a.kv.page_table + (size_t)item * a.kv.pages_per_seq;
-        const uint32_t pt = a.kv.page_tokens;
+        const uint32_t pt = a.kv.page_tokens, rowb = hd * sizeof(float);
+        const uint64_t pol = l2_evict_first_policy();
         int fault = 0;
-        constexpr uint32_t kNoRow = 0xFFFFFFFFu;
-        // lane l: the page of the warp's key l % 16 in tile t, and its row in the pools
-        auto page_of = [&](uint32_t t) -> int32_t {
-            const uint32_t at = t * kRowsKeys + 16 * cw + (lane & 15);
-            return t < t1 && at < places ? table[at / pt] : 0;
+        auto page_of = [&](uint32_t t, uint32_t h) -> int32_t {
+            const uint32_t at = (t0 + t) * kRowsKeys + lane + 32 * h;
+            return t < nt && at < places ? table[at / pt] : 0;
         };
-        auto row_of = [&](uint32_t t, int32_t page, bool &hidden) -> uint32_t {
-            const uint32_t at = t * kRowsKeys + 16 * cw + (lane & 15);
-            hidden = false;
-            if (t >= t1 || at >= places) return kNoRow;
-            if (page < 0 || (a.pool_pages != 0 && (uint32_t)page >= a.pool_pages)) {
-                fault = B2_ERR_POSITION;
-                hidden = true;
-                return kNoRow;
-            }
-            return ((uint32_t)page * a.n_kv_heads + kvh) * pt + at % pt;
-        };
-        // lanes 0..15 ask for their key's K row, 16..31 for its V row
-        auto ask = [&](uint32_t row) {
-            if (row == kNoRow) return;
-            const float *src = (lane < 16 ? a.kv.k_pool : a.kv.v_pool) + (size_t)row * hd;
-            for (uint32_t d = 0; d < hd; d += 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + d));
-        };
-        constexpr int U = HD / 4;  // values a lane holds of eight keys
-        // K: eight dimensions each of chunks ch, ch + 4, .. of key `key`
-        auto load_k = [&](float (&x)[U], uint32_t rows, uint32_t g) {
-            const uint32_t row = __shfl_sync(0xffffffffu, rows, 8 * g + key);
-            const float *src = a.kv.k_pool + (size_t)row * hd + 8 * ch;
+        int32_t page[2] = {page_of(0, 0), page_of(0, 1)};
+        uint32_t filled = 0;
+        bool ok = true;
+        for (uint32_t j = 0; ok && j < nt; ++j) {
+            size_t row[2];
+            uint32_t run[2], bytes = 0, bad[2];
 #pragma unroll
-            for (int i = 0; i < HD / 32; ++i) {
-                float4 u = make_float4(0, 0, 0, 0), v = u;
-                if (row != kNoRow && 32 * i + 8 * ch < hd) {
-                    u = *reinterpret_cast<const float4 *>(src + 32 * i);
-                    v = *reinterpret_cast<const float4 *>(src + 32 * i + 4);
+            for (uint32_t h = 0; h < 2; ++h) {
+                const uint32_t k = lane + 32 * h, at = (t0 + j) * kRowsKeys + k, off = at % pt;
+                const bool in = at < places;
+                const bool wrong = in && (page[h] < 0 || (a.pool_pages != 0 && (uint32_t)page[h] >= a.pool_pages));
+                bad[h] = __ballot_sync(0xffffffffu, wrong);
+                if (wrong) fault = B2_ERR_POSITION;
+                // a run: the tile's places on one page, copied by its first place's lane
+                const bool first = in && !wrong && (k == 0 || off == 0);
+                run[h] = first ? min(min(kRowsKeys - k, pt - off), places - at) : 0;
+                row[h] = (((size_t)(uint32_t)page[h] * a.n_kv_heads + kvh) * pt + off) * hd;
+                bytes += run[h] * rowb;
+                page[h] = page_of(j + 1, h);
+            }
+            bytes = __reduce_add_sync(0xffffffffu, bytes);
+#pragma unroll
+            for (uint32_t op = 0; op < 2 && ok; ++op) {
+                const uint32_t i = 2 * j + op, sl = i % NR;
+                if (i >= NR) ok = warp_wait(&r_empty[sl], i / NR - 1, a.err);
+                if (!ok) break;
+                if (lane == 0) {
+                    rhide[sl] = (uint64_t)bad[1] << 32 | bad[0];
+                    mbar_arrive_expect_tx(&r_full[sl], bytes);
                 }
-                x[8 * i] = u.x, x[8 * i + 1] = u.y, x[8 * i + 2] = u.z, x[8 * i + 3] = u.w;
-                x[8 * i + 4] = v.x, x[8 * i + 5] = v.y, x[8 * i + 6] = v.z, x[8 * i + 7] = v.w;
-            }
-        };
-        // V: dimensions lane + 32 i of the eight keys
-        auto load_v = [&](float (&x)[U], uint32_t rows, uint32_t g) {
+                __syncwarp();
+                const float *pool = op == 0 ? a.kv.k_pool : a.kv.v_pool;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const uint32_t row = __shfl_sync(0xffffffffu, rows, 8 * g + k);
-                const float *src = a.kv.v_pool + (size_t)row * hd + lane;
-#pragma unroll
-                for (int i = 0; i < HD / 32; ++i) x[8 * i + k] = row != kNoRow && lane + 32 * i < hd ? src[32 * i] : 0.0f;
+                for (uint32_t h = 0; h < 2; ++h)
+                    if (run[h] != 0)
+                        bulk_g2s_stream(smem + S::off_r + sl * S::slot + (lane + 32 * h) * rowb, pool + row[h], run[h] * rowb,
+                                        &r_full[sl], pol);
+                filled = i + 1;
             }
-        };
-        // largest magnitude of the eight keys (bits)
+        }
+        // no copy is in flight when the CTA ends, not even after a wait that gave up
+        for (uint32_t i = filled > NR ? filled - NR : 0; i < filled; ++i) warp_wait(&r_full[i % NR], i / NR, a.err);
+        if (fault) raise_error(a.err, fault);
+    } else if (warp >= (uint32_t)kRowsSoftWarps && warp < kRowsMmaWarp) {
+        // ---- ring tiles into operands ----
+        // Units of eight places' K or V, 16 to a tile (K 0..7, V 0..7), dealt to the
+        // warps in turn.
+        constexpr int U = HD / 4;  // values a lane holds of a unit
+        const uint32_t units = nt * 16, key = lane & 7;
         auto largest = [&](const float (&x)[U]) -> uint32_t {
             uint32_t top = 0;
 #pragma unroll
@@ -294,127 +317,150 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
             }
             return bad;
         };
-        // eight values in a row (K: dimensions of a key, V: keys of a dimension) are one 16-byte chunk
-        auto store = [&](const float (&x)[U], float sc, uint8_t *dst, uint32_t step, uint32_t lo_off, uint32_t first, uint32_t per) {
+        for (uint32_t u = warp - kRowsSoftWarps; u < units; u += kRowsConvWarps) {
+            const uint32_t j = u / 16, w = u & 7, i = u / 8, sl = i % NR;
+            if (!warp_wait(&r_full[sl], i / NR, a.err)) break;
+            const uint32_t place = (t0 + j) * kRowsKeys + 8 * w;
+            // places past the end (never copied) and on bad pages are zeros, hidden from every row
+            uint32_t none = (uint32_t)(rhide[sl] >> (8 * w)) & 0xFFu;
+            if (place + 8 > places) none |= places <= place ? 0xFFu : (0xFFu << (places - place)) & 0xFFu;
+            const float *src = reinterpret_cast<const float *>(smem + S::off_r + sl * S::slot) + (size_t)8 * w * hd;
+            float x[U];
+            if ((u & 8) == 0) {
+                // K: the lane's key is `key`, its chunks of eight dimensions c0, c0 + 4, ..; the
+                // rotation by the key and the swapped halves keep the reads of eight rows and the
+                // writes of one 16-byte column each free of bank conflicts
+                const uint32_t c0 = ((lane >> 3) + key) & 3, swap = key & 4;
 #pragma unroll
-            for (int i = 0; i < HD / 32; ++i) {
-                if (first + per * i < hd) {
-                    uint4 h, l;
-                    split_f16(x[8 * i] * sc, x[8 * i + 1] * sc, h.x, l.x);
-                    split_f16(x[8 * i + 2] * sc, x[8 * i + 3] * sc, h.y, l.y);
-                    split_f16(x[8 * i + 4] * sc, x[8 * i + 5] * sc, h.z, l.z);
-                    split_f16(x[8 * i + 6] * sc, x[8 * i + 7] * sc, h.w, l.w);
-                    *reinterpret_cast<uint4 *>(dst + i * step) = h;
-                    *reinterpret_cast<uint4 *>(dst + i * step + lo_off) = l;
+                for (int k = 0; k < HD / 32; ++k) {
+                    const uint32_t d = EXACT || 32 * k + 8 * c0 < hd ? 32 * k + 8 * c0 : 0;
+                    const float4 f = *reinterpret_cast<const float4 *>(src + key * hd + d + swap),
+                                 g = *reinterpret_cast<const float4 *>(src + key * hd + d + (swap ^ 4));
+                    x[8 * k] = f.x, x[8 * k + 1] = f.y, x[8 * k + 2] = f.z, x[8 * k + 3] = f.w;
+                    x[8 * k + 4] = g.x, x[8 * k + 5] = g.y, x[8 * k + 6] = g.z, x[8 * k + 7] = g.w;
                 }
+                if (none >> key & 1) {
+#pragma unroll
+                    for (int k = 0; k < U; ++k) x[k] = 0.0f;
+                }
+                uint32_t top = largest(x), mark = none << 8;
+                if (top >= 0x7F800000u) {
+                    const uint32_t who = __ballot_sync(0xffffffffu, drop_bad(x) != 0);
+                    mark |= (who | who >> 8 | who >> 16 | who >> 24) & 0xFFu;
+                    top = largest(x);
+                }
+                if (lane == 0) mbar_arrive(&r_empty[sl]);  // every lane's values are in registers
+                const uint32_t st = j % KST;
+                if (j >= KST && !warp_wait(&k_empty[st], j / KST - 1, a.err)) break;
+                const int e = top_exp(top);
+                const float sc = pow2i(kRowsTop - e);
+                // element (key, d): chunk d / 8 of 64 rows
+                uint8_t *dst = smem + S::off_k + st * 2 * S::half + c0 * (kRowsKeys * 16) + w * 128 + key * 16;
+#pragma unroll
+                for (int k = 0; k < HD / 32; ++k) {
+                    if (EXACT || 32 * k + 8 * c0 < hd) {
+                        uint2 h0, h1, l0, l1;
+                        split_f16(x[8 * k] * sc, x[8 * k + 1] * sc, h0.x, l0.x);
+                        split_f16(x[8 * k + 2] * sc, x[8 * k + 3] * sc, h0.y, l0.y);
+                        split_f16(x[8 * k + 4] * sc, x[8 * k + 5] * sc, h1.x, l1.x);
+                        split_f16(x[8 * k + 6] * sc, x[8 * k + 7] * sc, h1.y, l1.y);
+                        *reinterpret_cast<uint4 *>(dst + k * 4 * (kRowsKeys * 16)) =
+                            swap ? make_uint4(h1.x, h1.y, h0.x, h0.y) : make_uint4(h0.x, h0.y, h1.x, h1.y);
+                        *reinterpret_cast<uint4 *>(dst + k * 4 * (kRowsKeys * 16) + S::half) =
+                            swap ? make_uint4(l1.x, l1.y, l0.x, l0.y) : make_uint4(l0.x, l0.y, l1.x, l1.y);
+                    }
+                }
+                if (lane == 0) {
+                    kscale[(j % kRowsMeta) * 8 + w] = pow2i(e - kRowsTop);
+                    kmark[(j % kRowsMeta) * 8 + w] = mark;
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&k_full[st]);
+            } else {
+                // V: dimensions lane + 32 k of the eight places
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+#pragma unroll
+                    for (int k = 0; k < HD / 32; ++k)
+                        x[8 * k + c] = src[c * hd + (EXACT || lane + 32 * k < hd ? lane + 32 * k : 0)];
+                if (none != 0) {
+#pragma unroll
+                    for (int k = 0; k < U; ++k)
+                        if (none >> (k & 7) & 1) x[k] = 0.0f;
+                }
+                uint32_t top = largest(x), mark = 0;
+                if (top >= 0x7F800000u) {
+                    mark = __reduce_or_sync(0xffffffffu, drop_bad(x));
+                    top = largest(x);
+                }
+                if (lane == 0) mbar_arrive(&r_empty[sl]);
+                const uint32_t st = j % VST;
+                if (j >= VST && !warp_wait(&v_empty[st], j / VST - 1, a.err)) break;
+                const int e = top_exp(top);
+                const float sc = pow2i(kRowsTop - e);
+                // element (d, place): chunk place / 8 of HD rows
+                uint8_t *dst = smem + S::off_v + st * 2 * S::half + w * (HD * 16) + lane * 16;
+#pragma unroll
+                for (int k = 0; k < HD / 32; ++k) {
+                    if (EXACT || lane + 32 * k < hd) {
+                        uint4 h, l;
+                        split_f16(x[8 * k] * sc, x[8 * k + 1] * sc, h.x, l.x);
+                        split_f16(x[8 * k + 2] * sc, x[8 * k + 3] * sc, h.y, l.y);
+                        split_f16(x[8 * k + 4] * sc, x[8 * k + 5] * sc, h.z, l.z);
+                        split_f16(x[8 * k + 6] * sc, x[8 * k + 7] * sc, h.w, l.w);
+                        *reinterpret_cast<uint4 *>(dst + k * 512) = h;
+                        *reinterpret_cast<uint4 *>(dst + k * 512 + S::half) = l;
+                    }
+                }
+                if (lane == 0) {
+                    vexp[st * 8 + w] = e;
+                    vmark[st * 8 + w] = mark;
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_full[st]);
             }
-        };
-        auto convert_k = [&](float (&x)[U], uint32_t j, uint32_t g, uint32_t hide) {
-            const uint32_t w = 2 * cw + g;
-            uint32_t top = largest(x), mark = (hide >> (8 * g) & 0xFFu) << 8;
-            if (top >= 0x7F800000u) {
-                const uint32_t who = __ballot_sync(0xffffffffu, drop_bad(x) != 0);
-                mark |= (who | who >> 8 | who >> 16 | who >> 24) & 0xFFu;
-                top = largest(x);
-            }
-            const int e = top_exp(top);
-            // element (key, d): chunk d / 8 of 128 rows (hi rows 0..63, lo rows 64..127)
-            store(x, pow2i(kRowsTop - e), smem + S::off_k + (j % NST) * S::k_stage + ch * (2 * kRowsKeys * 16) + w * 128 + key * 16,
-                  4 * (2 * kRowsKeys * 16), kRowsKeys * 16, 8 * ch, 32);
-            if (lane == 0) {
-                kscale[(j % kRowsMeta) * 8 + w] = pow2i(e - kRowsTop);
-                kmark[(j % kRowsMeta) * 8 + w] = mark;
-            }
-        };
-        auto convert_v = [&](float (&x)[U], uint32_t j, uint32_t g) {
-            const uint32_t w = 2 * cw + g;
-            uint32_t top = largest(x), mark = 0;
-            if (top >= 0x7F800000u) {
-                mark = __reduce_or_sync(0xffffffffu, drop_bad(x));
-                top = largest(x);
-            }
-            const int e = top_exp(top);
-            // element (d, key): chunk key / 8 of HD rows
-            store(x, pow2i(kRowsTop - e), smem + S::off_v + (j % NST) * 2 * S::v_half + w * (HD * 16) + lane * 16, 512, S::v_half, lane, 32);
-            if (lane == 0) {
-                vexp[(j % NST) * 8 + w] = e;
-                vmark[(j % NST) * 8 + w] = mark;
-            }
-        };
-        auto publish = [&](uint64_t *bar) {
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar);
-        };
-        bool hidden, unused;
-        uint32_t rows = row_of(t0, page_of(t0), hidden);
-        ask(rows);
-        float xa[U], xb[U];
-        load_k(xa, rows, 0);
-        for (uint32_t i = 1; i < kRowsAhead; ++i) ask(row_of(t0 + i, page_of(t0 + i), unused));
-        int32_t page = page_of(t0 + 1), far = page_of(t0 + kRowsAhead);
-        for (uint32_t j = 0; j < nt; ++j) {
-            const uint32_t st = j % NST, pass = j / NST, hide = __ballot_sync(0xffffffffu, hidden);
-            load_k(xb, rows, 1);
-            ask(row_of(t0 + j + kRowsAhead, far, unused));
-            far = page_of(t0 + j + 1 + kRowsAhead);
-            if (j >= NST && !warp_wait(&k_empty[st], pass - 1, a.err)) break;
-            convert_k(xa, j, 0, hide);
-            load_v(xa, rows, 0);
-            convert_k(xb, j, 1, hide);
-            publish(&k_full[st]);
-            load_v(xb, rows, 1);
-            if (j >= NST && !warp_wait(&v_empty[st], pass - 1, a.err)) break;
-            convert_v(xa, j, 0);
-            if (j + 1 < nt) {  // K of the next tile on its way while V is converted
-                rows = row_of(t0 + j + 1, page, hidden);
-                page = page_of(t0 + j + 2);
-                load_k(xa, rows, 0);
-            }
-            convert_v(xb, j, 1);
-            publish(&v_full[st]);
         }
-        if (fault) raise_error(a.err, fault);
-    } else if (warp == kRowsSoftWarps + kRowsConvWarps) {
+    } else if (warp == kRowsMmaWarp) {
         // ---- MMA issue ----
         if (lane == 0) {
-            const uint32_t id_s2 = umma_idesc_f16(kRowsM, 2 * kRowsKeys), id_s1 = umma_idesc_f16(kRowsM, kRowsKeys);
-            const uint32_t id_o = umma_idesc_f16(kRowsM, hd);
-            const uint32_t qb = smem_u32(smem + S::off_q), kb = smem_u32(smem + S::off_k), vb = smem_u32(smem + S::off_v),
-                           pb = smem_u32(smem + S::off_p);
+            const uint32_t id_s = umma_idesc_f16(kRowsM, kRowsKeys), id_o = umma_idesc_f16(kRowsM, hd);
+            const uint32_t kb = smem_u32(smem + S::off_k), vb = smem_u32(smem + S::off_v);
             bool ok = mbar_wait_bounded(q_full, 0, a.err);
             for (uint32_t j = 0; ok && j <= nt; ++j) {
                 if (j < nt) {  // S of tile j
-                    const uint32_t st = j % NST, sb = j & 1;
-                    ok = mbar_wait_bounded(&k_full[st], (j / NST) & 1, a.err) &&
-                         (j < 2 || mbar_wait_bounded(&s_empty[sb], (j / 2 - 1) & 1, a.err));
+                    const uint32_t st = j % KST;
+                    ok = mbar_wait_bounded(&k_full[st], (j / KST) & 1, a.err) &&
+                         (j == 0 || mbar_wait_bounded(s_empty, (j - 1) & 1, a.err));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t d = tmem + sb * 2 * kRowsKeys, kt = kb + st * S::k_stage;
+                    const uint32_t kt = kb + st * 2 * S::half;
+#pragma unroll 4
                     for (uint32_t kk = 0; kk < hd / 16; ++kk) {
-                        const uint64_t b = umma_desc(kt + kk * 2 * (2 * kRowsKeys * 16), 2 * kRowsKeys * 16, 128);
-                        umma_16(d, umma_desc(qb + kk * 2 * (kRowsM * 16), kRowsM * 16, 128), b, id_s2, kk > 0);
-                        umma_16(d, umma_desc(qb + S::q_half + kk * 2 * (kRowsM * 16), kRowsM * 16, 128), b, id_s1, 1);
+                        const uint64_t kh = umma_desc(kt + kk * 2 * (kRowsKeys * 16), kRowsKeys * 16, 128);
+                        const uint64_t kl = umma_desc(kt + S::half + kk * 2 * (kRowsKeys * 16), kRowsKeys * 16, 128);
+                        umma_16_ts(tm_s, tm_q + kk * 8, kh, id_s, kk > 0);
+                        umma_16_ts(tm_s, tm_q + HD / 2 + kk * 8, kh, id_s, 1);
+                        umma_16_ts(tm_s, tm_q + kk * 8, kl, id_s, 1);
                     }
-                    umma_commit(&s_full[sb]);
+                    umma_commit(s_full);
                     umma_commit(&k_empty[st]);
                 }
                 if (j > 0) {  // O of tile j - 1
-                    const uint32_t i = j - 1, st = i % NST, ob = i & 1;
-                    ok = mbar_wait_bounded(p_full, i & 1, a.err) && mbar_wait_bounded(&v_full[st], (i / NST) & 1, a.err) &&
+                    const uint32_t i = j - 1, st = i % VST, ob = i & 1;
+                    ok = mbar_wait_bounded(p_full, i & 1, a.err) && mbar_wait_bounded(&v_full[st], (i / VST) & 1, a.err) &&
                          (i < 2 || mbar_wait_bounded(&o_empty[ob], (i / 2 - 1) & 1, a.err));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t d = tmem + 4 * kRowsKeys + ob * HD, vt = vb + st * 2 * S::v_half;
+                    const uint32_t d = tm_o + ob * HD, vt = vb + st * 2 * S::half;
 #pragma unroll
                     for (uint32_t kk = 0; kk < kRowsKeys / 16; ++kk) {
-                        const uint64_t ph = umma_desc(pb + kk * 2 * (kRowsM * 16), kRowsM * 16, 128);
-                        const uint64_t pl = umma_desc(pb + S::p_half + kk * 2 * (kRowsM * 16), kRowsM * 16, 128);
                         const uint64_t vh = umma_desc(vt + kk * 2 * (HD * 16), HD * 16, 128);
-                        const uint64_t vl = umma_desc(vt + S::v_half + kk * 2 * (HD * 16), HD * 16, 128);
-                        umma_16(d, ph, vh, id_o, kk > 0);
-                        umma_16(d, pl, vh, id_o, 1);
-                        umma_16(d, ph, vl, id_o, 1);
+                        const uint64_t vl = umma_desc(vt + S::half + kk * 2 * (HD * 16), HD * 16, 128);
+                        umma_16_ts(d, tm_p + kk * 8, vh, id_o, kk > 0);
+                        umma_16_ts(d, tm_p + 32 + kk * 8, vh, id_o, 1);
+                        umma_16_ts(d, tm_p + kk * 8, vl, id_o, 1);
                     }
                     umma_commit(&o_full[ob]);
                     umma_commit(&v_empty[st]);
@@ -428,63 +474,39 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
     } else {
         const uint32_t qt = warp & 3, half = warp >> 2;
         if (qt < nsoft / 2) {
-            // ---- softmax and the sums of O: row r, keys 32 half .. + 31, dimensions of half ----
+            // ---- softmax and the sums of O: row r, places 32 half .. + 31, dimensions of half ----
             const uint32_t r = qt * 32 + lane, m_row = blk * kRowsM + r;
             const bool mine = r < live;
             const uint32_t tok = mine ? m_row / p.group : 0, head = kvh * p.group + (mine ? m_row % p.group : 0);
             const uint32_t lanes = (qt * 32) << 16;
-            uint32_t xph = 0;  // exchanges done with the other half's warp
-            auto exchange = [&](float mine_v, float &other) -> bool {
-                float *x = xmax + (xph & 1) * 2 * kRowsM;
-                x[half * kRowsM + r] = mine_v;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&xbar[qt]);
-                const bool ok = warp_wait(&xbar[qt], xph, a.err);
-                other = x[(half ^ 1) * kRowsM + r];
-                ++xph;
-                return ok;
-            };
             float cq;  // score of a row: dot * K scale * cq, in powers of two
-            bool ok;
             {
                 const float *src = a.q + (size_t)(r0 + tok) * a.q_stride + (size_t)head * hd;
-                float x[HD / 2];
                 uint32_t top = 0;
-#pragma unroll
-                for (int c = 0; c < HD / 16; ++c) {
-                    const uint32_t d = half * (HD / 2) + 8 * c;
-                    float4 u = make_float4(0, 0, 0, 0), v = u;
-                    if (mine && d < hd) {
-                        u = *reinterpret_cast<const float4 *>(src + d);
-                        v = *reinterpret_cast<const float4 *>(src + d + 4);
-                    }
-                    x[8 * c] = u.x, x[8 * c + 1] = u.y, x[8 * c + 2] = u.z, x[8 * c + 3] = u.w;
-                    x[8 * c + 4] = v.x, x[8 * c + 5] = v.y, x[8 * c + 6] = v.z, x[8 * c + 7] = v.w;
+                for (uint32_t d = 0; mine && d < hd; d += 4) {  // the row's largest magnitude
+                    const float4 f = *reinterpret_cast<const float4 *>(src + d);
+                    top = max(max(top, max(abs_bits(f.x), abs_bits(f.y))), max(abs_bits(f.z), abs_bits(f.w)));
                 }
-#pragma unroll
-                for (int i = 0; i < HD / 2; ++i) top = max(top, abs_bits(x[i]));
-                float other;
-                ok = exchange(__uint_as_float(top), other);
-                top = max(top, __float_as_uint(other));
                 const bool bad = top >= 0x7F800000u;
                 const int e = bad ? 0 : top_exp(top);
-                const float sc = bad ? 0.0f : pow2i(kRowsTop - e);
+                const float sc = pow2i(kRowsTop - e);
                 cq = bad ? NAN : pow2i(e - kRowsTop) * p.scale;
-                uint8_t *dst = smem + S::off_q + r * 16;
 #pragma unroll
-                for (int c = 0; c < HD / 16; ++c) {
-                    const uint32_t chunk = half * (HD / 16) + c;
-                    uint4 h = make_uint4(0, 0, 0, 0), l = h;
-                    if (!bad) {
-                        split_f16(x[8 * c] * sc, x[8 * c + 1] * sc, h.x, l.x);
-                        split_f16(x[8 * c + 2] * sc, x[8 * c + 3] * sc, h.y, l.y);
-                        split_f16(x[8 * c + 4] * sc, x[8 * c + 5] * sc, h.z, l.z);
-                        split_f16(x[8 * c + 6] * sc, x[8 * c + 7] * sc, h.w, l.w);
+                for (uint32_t c = 0; c < HD / 2; c += 32) {  // 32 dimensions: 16 columns of hi, 16 of lo
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; ++k) {
+                        const uint32_t d = half * (HD / 2) + c + 4 * k;
+                        float4 f = make_float4(0, 0, 0, 0);
+                        if (mine && !bad && d < hd) f = *reinterpret_cast<const float4 *>(src + d);
+                        split_f16(f.x * sc, f.y * sc, hi[2 * k], lo[2 * k]);
+                        split_f16(f.z * sc, f.w * sc, hi[2 * k + 1], lo[2 * k + 1]);
                     }
-                    *reinterpret_cast<uint4 *>(dst + chunk * (kRowsM * 16)) = h;
-                    *reinterpret_cast<uint4 *>(dst + chunk * (kRowsM * 16) + S::q_half) = l;
+                    tmem_st16(tm_q + lanes + half * (HD / 4) + c / 2, hi);
+                    tmem_st16(tm_q + lanes + HD / 2 + half * (HD / 4) + c / 2, lo);
                 }
-                fence_proxy_async();
+                tmem_wait_st();
+                tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full);
             }
@@ -495,48 +517,30 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
             for (int i = 0; i < HD / 2; ++i) acc[i] = 0.0f;
             // O of tile i into the sums: acc = acc * corr + O * osc
             auto take_o = [&](uint32_t i) {
-                const uint32_t col = tmem + lanes + 4 * kRowsKeys + (i & 1) * HD + half * (HD / 2);
+                const uint32_t col = tm_o + lanes + (i & 1) * HD + half * (HD / 2);
                 tc_fence_after();
+                if (!__all_sync(0xffffffffu, corr_prev == 1.0f || !mine)) {
 #pragma unroll
-                for (int c = 0; c < HD / 2; c += 16) {
-                    uint32_t v[16];
+                    for (int k = 0; k < HD / 2; ++k) acc[k] *= corr_prev;
+                }
+#pragma unroll
+                for (int c = 0; c < HD / 2; c += 32) {
+                    uint32_t v[16], w[16];
                     tmem_ld16_nowait(col + c, v);
+                    tmem_ld16_nowait(col + c + 16, w);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) acc[c + k] = fmaf(__uint_as_float(v[k]), osc_prev, acc[c + k] * corr_prev);
+                    for (int k = 0; k < 16; ++k) {
+                        acc[c + k] = fmaf(__uint_as_float(v[k]), osc_prev, acc[c + k]);
+                        acc[c + 16 + k] = fmaf(__uint_as_float(w[k]), osc_prev, acc[c + 16 + k]);
+                    }
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&o_empty[i & 1]);
             };
-            uint32_t j = 0;
-            for (; ok && j < nt; ++j) {
-                const uint32_t sb = j & 1, mt = j % kRowsMeta, vt = j % NST;
-                ok = warp_wait(&s_full[sb], j / 2, a.err) && warp_wait(&v_full[vt], j / NST, a.err);
-                if (!ok) break;
-                tc_fence_after();
-                float s[32];
-                const float4 ks = *reinterpret_cast<const float4 *>(kscale + mt * 8 + half * 4);
-                const float ksc[4] = {ks.x, ks.y, ks.z, ks.w};
-                const uint4 km = *reinterpret_cast<const uint4 *>(kmark + mt * 8 + half * 4);
-                const uint4 vm = *reinterpret_cast<const uint4 *>(vmark + vt * 8 + half * 4);
-                const int4 e0 = *reinterpret_cast<const int4 *>(vexp + vt * 8), e1 = *reinterpret_cast<const int4 *>(vexp + vt * 8 + 4);
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t u[16], v[16];
-                    const uint32_t col = tmem + lanes + sb * 2 * kRowsKeys + half * 32 + c * 16;
-                    tmem_ld16_nowait(col, u);
-                    tmem_ld16_nowait(col + kRowsKeys, v);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int k = 0; k < 16; ++k)
-                        s[c * 16 + k] = (__uint_as_float(u[k]) + __uint_as_float(v[k])) * ksc[(c * 16 + k) / 8];
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s_empty[sb]);
-                // keys this row does not see, and keys whose K or V is not finite
-                const uint32_t key0 = (t0 + j) * kRowsKeys + half * 32;
+            // places of the 32 from key0 that this row sees
+            auto visible = [&](uint32_t key0) -> uint32_t {
                 uint32_t vis = 0xFFFFFFFFu;
                 if (key0 + 32 > ctx) {
                     if (a.tree != nullptr) {
@@ -553,58 +557,99 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                     }
                 }
                 if (key0 + 32 > places) vis &= places <= key0 ? 0 : (1u << (places - key0)) - 1;
-                const uint32_t any = km.x | km.y | km.z | km.w | vm.x | vm.y | vm.z | vm.w;
-                if (any != 0) {
-                    const uint32_t bad = ((km.x | vm.x) & 0xFF) | ((km.y | vm.y) & 0xFF) << 8 | ((km.z | vm.z) & 0xFF) << 16 |
-                                         ((km.w | vm.w) & 0xFF) << 24;
-                    vis &= ~((km.x >> 8) | (km.y >> 8) << 8 | (km.z >> 8) << 16 | (km.w >> 8) << 24);
-#pragma unroll
-                    for (int k = 0; k < 32; ++k)
-                        if (bad >> k & 1) s[k] = NAN;
-                }
-                if (vis != 0xFFFFFFFFu) {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k)
-                        if (!(vis >> k & 1)) s[k] = -INFINITY;
-                }
-                float top = s[0];
-#pragma unroll
-                for (int k = 1; k < 32; ++k) top = fmaxf(top, s[k]);
-                float other;
-                ok = exchange(top, other);
+                return vis;
+            };
+            bool ok = true;
+            for (uint32_t j = 0; j < nt; ++j) {
+                const uint32_t mt = j % kRowsMeta, vt = j % VST;
+                ok = warp_wait(s_full, j, a.err);
                 if (!ok) break;
-                const float m_new = fmaxf(m, fmaxf(top, other) * cq);
-                const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-                const float corr = ex2(m - m_use), shift = kRowsP - m_use;
-                const int emax = max(max(max(e0.x, e0.y), max(e0.z, e0.w)), max(max(e1.x, e1.y), max(e1.z, e1.w)));
-                const int4 eh = half ? e1 : e0;
-                const int eg[4] = {eh.x, eh.y, eh.z, eh.w};
-                float sum = 0.0f;
-                uint32_t hi[16], lo[16];
+                tc_fence_after();
+                float s[32], top = -INFINITY;
+                // the other half's scores, for the maximum alone, then this half's
+                float ks0 = 0.0f;
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const float f = pow2i(max(eg[g] - emax, -126));
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float p0 = ex2(fmaf(s[8 * g + 2 * k], cq, shift)), p1 = ex2(fmaf(s[8 * g + 2 * k + 1], cq, shift));
-                        sum += p0 + p1;
-                        split_f16(p0 * f, p1 * f, hi[4 * g + k], lo[4 * g + k]);
+                for (int o = 0; o < 2; ++o) {
+                    const uint32_t hh = o == 0 ? half ^ 1 : half;
+                    const float4 ks = *reinterpret_cast<const float4 *>(kscale + mt * 8 + hh * 4);
+                    const uint4 km = *reinterpret_cast<const uint4 *>(kmark + mt * 8 + hh * 4);
+                    uint32_t u[16], v[16];
+                    tmem_ld16_nowait(tm_s + lanes + hh * 32, u);
+                    tmem_ld16_nowait(tm_s + lanes + hh * 32 + 16, v);
+                    tmem_wait_ld();
+                    if (o == 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(s_empty);
                     }
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        s[k] = __uint_as_float(u[k]);
+                        s[16 + k] = __uint_as_float(v[k]);
+                    }
+                    ks0 = fmaxf(fmaxf(ks.x, ks.y), fmaxf(ks.z, ks.w));
+                    if (ks.x != ks0 || ks.y != ks0 || ks.z != ks0 || ks.w != ks0) {  // units of different scale: to the largest
+                        const float f[4] = {ks.x / ks0, ks.y / ks0, ks.z / ks0, ks.w / ks0};
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) s[k] *= f[k / 8];
+                    }
+                    uint32_t vis = visible((t0 + j) * kRowsKeys + hh * 32);
+                    if ((km.x | km.y | km.z | km.w) != 0) {
+                        const uint32_t bad = (km.x & 0xFF) | (km.y & 0xFF) << 8 | (km.z & 0xFF) << 16 | (km.w & 0xFF) << 24;
+                        vis &= ~((km.x >> 8) | (km.y >> 8) << 8 | (km.z >> 8) << 16 | (km.w >> 8) << 24);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (bad >> k & 1) s[k] = NAN;
+                    }
+                    if (vis != 0xFFFFFFFFu) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (!(vis >> k & 1)) s[k] = -INFINITY;
+                    }
+                    float t = s[0];
+#pragma unroll
+                    for (int k = 1; k < 32; ++k) t = fmaxf(t, s[k]);
+                    top = fmaxf(top, t * ks0);
+                }
+                const float m_new = fmaxf(m, top * cq);
+                const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+                const float corr = ex2(m - m_use), shift = kRowsP - m_use, cqk = cq * ks0;
+                float sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                    s[k] = ex2(fmaf(s[k], cqk, shift));
+                    sum += s[k];
                 }
                 l = fmaf(l, corr, sum);
                 m = m_new;
+                ok = warp_wait(&v_full[vt], j / VST, a.err);
+                if (!ok) break;
+                const int4 e0 = *reinterpret_cast<const int4 *>(vexp + vt * 8), e1 = *reinterpret_cast<const int4 *>(vexp + vt * 8 + 4);
+                const uint4 vm = *reinterpret_cast<const uint4 *>(vmark + vt * 8 + half * 4);
+                const int emax = max(max(max(e0.x, e0.y), max(e0.z, e0.w)), max(max(e1.x, e1.y), max(e1.z, e1.w)));
+                const int4 eh = half ? e1 : e0;
+                if ((eh.x & eh.y & eh.z & eh.w) != emax || (eh.x | eh.y | eh.z | eh.w) != emax) {  // not all the tile's largest
+                    const int eg[4] = {eh.x, eh.y, eh.z, eh.w};
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) s[k] *= pow2i(max(eg[k / 8] - emax, -126));
+                }
+                if ((vm.x | vm.y | vm.z | vm.w) != 0) {  // a NaN or infinity in V reaches the rows that see its place
+                    const uint32_t bad = (vm.x & 0xFF) | (vm.y & 0xFF) << 8 | (vm.z & 0xFF) << 16 | (vm.w & 0xFF) << 24;
+                    const uint32_t hit = bad & visible((t0 + j) * kRowsKeys + half * 32);
+                    if (hit != 0) l = NAN;
+                }
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) split_f16(s[2 * k], s[2 * k + 1], hi[k], lo[k]);
                 if (j > 0) {
                     ok = warp_wait(&o_full[(j - 1) & 1], (j - 1) / 2, a.err);  // P is free, and O of tile j - 1 is there
                     if (!ok) break;
+                    tc_fence_after();
                 }
-                uint8_t *dst = smem + S::off_p + half * 4 * (kRowsM * 16) + r * 16;
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    *reinterpret_cast<uint4 *>(dst + g * (kRowsM * 16)) = make_uint4(hi[4 * g], hi[4 * g + 1], hi[4 * g + 2], hi[4 * g + 3]);
-                    *reinterpret_cast<uint4 *>(dst + g * (kRowsM * 16) + S::p_half) =
-                        make_uint4(lo[4 * g], lo[4 * g + 1], lo[4 * g + 2], lo[4 * g + 3]);
-                }
-                fence_proxy_async();
+                tmem_st16(tm_p + lanes + half * 16, hi);
+                tmem_st16(tm_p + lanes + 32 + half * 16, lo);
+                tmem_wait_st();
+                tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full);
                 if (j > 0) take_o(j - 1);
@@ -614,9 +659,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
             if (ok) ok = warp_wait(&o_full[(nt - 1) & 1], (nt - 1) / 2, a.err);
             if (ok) {
                 take_o(nt - 1);
-                float other;
-                ok = exchange(l, other);
-                l = (half ? other : l) + (half ? l : other);  // the halves in one order
+                // the row's sum: both halves', in one order
+                xsum[half * kRowsM + r] = l;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&xbar[qt]);
+                ok = warp_wait(&xbar[qt], 0, a.err);
+                l = xsum[r] + xsum[kRowsM + r];
             }
             if (ok && mine) {
                 // the weights carry 2^12, the sums of O do not
@@ -645,7 +693,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kRowsSoftWarps + kRowsConvWarps) {
+    if (warp == kRowsMmaWarp) {
         tc_fence_after();
         tmem_free(tmem, 512);
     }
@@ -806,7 +854,10 @@ extern "C" int b2_attn_rows(const b2_attn_rows_args *a, void *stream)
     p.scale = (float)(1.4426950408889634 / sqrt((double)a->head_dim));
     const cudaStream_t st = (cudaStream_t)stream;
     const bool wide = a->head_dim > 64;
-    const void *fn = wide ? (const void *)attn_rows_kernel<128> : (const void *)attn_rows_kernel<64>;
+    const void *fn = a->head_dim == 128  ? (const void *)attn_rows_kernel<128, true>
+                     : wide              ? (const void *)attn_rows_kernel<128, false>
+                     : a->head_dim == 64 ? (const void *)attn_rows_kernel<64, true>
+                                         : (const void *)attn_rows_kernel<64, false>;
     const size_t smem = wide ? RowsSmem<128>::bytes : RowsSmem<64>::bytes;
     if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return -8;
     if (launch_rows_attn(fn, dim3(p.splits, a->n_kv_heads * p.blocks, a->batch), kRowsThreads, smem, a->pdl, st, p) != cudaSuccess)

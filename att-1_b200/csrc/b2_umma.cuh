@@ -40,6 +40,18 @@ __device__ __forceinline__ void umma_16(uint32_t tmem_d, uint64_t a, uint64_t b,
         : "memory");
 }
 
+// The same with A from tensor memory: row i in lane i, two 16-bit elements of a
+// row to a column (8 columns of one K = 16 MMA).
+__device__ __forceinline__ void umma_16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
 // Arrives on `bar` once every tcgen05 operation issued so far by this thread is complete.
 __device__ __forceinline__ void umma_commit(uint64_t *bar)
 {
