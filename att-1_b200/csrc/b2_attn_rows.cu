@@ -72,14 +72,12 @@ struct RowsSmem {
     static constexpr uint32_t off_k = 0;
     static constexpr uint32_t off_v = off_k + k_stages * 2 * half;
     static constexpr uint32_t off_r = off_v + v_stages * 2 * half;
-    static constexpr uint32_t off_x = off_r + slots * slot;         // [2][128] f32: the halves' sums
-    static constexpr uint32_t off_ks = off_x + 2 * kRowsM * 4;      // [kRowsMeta][8] f32: 1 / K scale of a unit
-    static constexpr uint32_t off_km = off_ks + kRowsMeta * 8 * 4;  // [kRowsMeta][8] u32: places that are NaN | hidden << 8
-    static constexpr uint32_t off_ve = off_km + kRowsMeta * 8 * 4;  // [2][8] int: exponent of a unit's V
-    static constexpr uint32_t off_vm = off_ve + 2 * 8 * 4;          // [2][8] u32: places whose V is NaN
+    static constexpr uint32_t off_x = off_r + slots * slot;         // [2][2][128] f32: the halves' maxima, by tile parity
+    static constexpr uint32_t off_km = off_x + 4 * kRowsM * 4;      // [kRowsMeta][8] u32: a K unit's exponent and marks
+    static constexpr uint32_t off_vm = off_km + kRowsMeta * 8 * 4;  // [2][8] u32: the same of V
     static constexpr uint32_t off_rh = off_vm + 2 * 8 * 4;          // [slots] u64: places whose page is bad
     static constexpr uint32_t off_bar = off_rh + 8 * slots;
-    static constexpr uint32_t bytes = off_bar + 8 * (2 * slots + 2 * k_stages + 2 * v_stages + 13) + 16;
+    static constexpr uint32_t bytes = off_bar + 8 * (2 * slots + 2 * k_stages + 2 * v_stages + 9) + 16;
 };
 static_assert(RowsSmem<128>::bytes <= 227 * 1024 && RowsSmem<64>::bytes <= 227 * 1024, "shared memory");
 
@@ -140,16 +138,63 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
+// What the softmax needs to know of a unit: exponent, places hidden from every
+// row, places with a NaN or infinity.
+__device__ __forceinline__ uint32_t unit_meta(int e, uint32_t hidden, uint32_t bad) { return (uint32_t)(e + 128) << 16 | hidden << 8 | bad; }
+__device__ __forceinline__ int meta_exp(uint32_t m) { return (int)(m >> 16) - 128; }
+// byte i of the result: (m_i >> shift) & 0xFF
+__device__ __forceinline__ uint32_t meta_bytes(const uint4 &m, uint32_t shift)
+{
+    return (m.x >> shift & 0xFF) | (m.y >> shift & 0xFF) << 8 | (m.z >> shift & 0xFF) << 16 | (m.w >> shift & 0xFF) << 24;
+}
+// Four units that share an exponent and have nothing marked.
+__device__ __forceinline__ bool meta_plain(const uint4 &m) { return m.x == m.y && m.x == m.z && m.x == m.w && (m.x & 0xFFFF) == 0; }
+
+// Two f32 in one register pair.
+__device__ __forceinline__ uint64_t pair(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// The same of two values scaled by the pair sc2.
+__device__ __forceinline__ void split_scaled(float a, float b, uint64_t sc2, uint32_t &hi, uint32_t &lo)
+{
+    float x, y;
+    unpair(mul2(pair(a, b), sc2), x, y);
+    split_f16(x, y, hi, lo);
+}
+
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
-__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16])
+// 32 lanes x 32 columns: thread i gets lane (base + i), columns col..col+31. The
+// registers hold after tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
 {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr)
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16])
 {
@@ -178,17 +223,14 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t split = blockIdx.x, kvh = blockIdx.y / p.blocks, blk = blockIdx.y % p.blocks, item = blockIdx.z;
     const uint32_t hd = EXACT ? HD : a.head_dim;  // EXACT: head_dim == HD
-    float *xsum = reinterpret_cast<float *>(smem + S::off_x);
-    float *kscale = reinterpret_cast<float *>(smem + S::off_ks);
-    uint32_t *kmark = reinterpret_cast<uint32_t *>(smem + S::off_km);
-    int *vexp = reinterpret_cast<int *>(smem + S::off_ve);
-    uint32_t *vmark = reinterpret_cast<uint32_t *>(smem + S::off_vm);
+    float *xmax = reinterpret_cast<float *>(smem + S::off_x);
+    uint32_t *kmeta = reinterpret_cast<uint32_t *>(smem + S::off_km), *vmeta = reinterpret_cast<uint32_t *>(smem + S::off_vm);
     uint64_t *rhide = reinterpret_cast<uint64_t *>(smem + S::off_rh);
     uint64_t *r_full = reinterpret_cast<uint64_t *>(smem + S::off_bar), *r_empty = r_full + NR, *k_full = r_empty + NR,
              *k_empty = k_full + KST, *v_full = k_empty + KST, *v_empty = v_full + VST, *s_full = v_empty + VST,
              *s_empty = s_full + 1, *p_full = s_empty + 1, *o_full = p_full + 1, *o_empty = o_full + 2, *q_full = o_empty + 2,
-             *done = q_full + 1, *xbar = done + 1;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(xbar + 4);
+             *done = q_full + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
 
     pdl_wait();
     pdl_launch_dependents();
@@ -229,7 +271,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
         }
         mbar_init(q_full, nsoft);
         mbar_init(done, 1);
-        for (uint32_t i = 0; i < 4; ++i) mbar_init(&xbar[i], 2);
         fence_mbar_init();
     }
     if (warp == kRowsMmaWarp) tmem_alloc(tmem_slot, 512);
@@ -296,130 +337,96 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
     } else if (warp >= (uint32_t)kRowsSoftWarps && warp < kRowsMmaWarp) {
         // ---- ring tiles into operands ----
         // Units of eight places' K or V, 16 to a tile (K 0..7, V 0..7), dealt to the
-        // warps in turn.
+        // warps in turn. K and V differ in how a lane picks its values; the conversion of
+        // its HD / 32 chunks of eight (16 bytes of hi, 16 of lo) is one piece of code for
+        // both: the roles of this kernel run different code side by side, and instruction
+        // fetch is what they run out of first.
         constexpr int U = HD / 4;  // values a lane holds of a unit
         const uint32_t units = nt * 16, key = lane & 7;
-        auto largest = [&](const float (&x)[U]) -> uint32_t {
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < U; ++i) top = max(top, abs_bits(x[i]));
-            return __reduce_max_sync(0xffffffffu, top);
-        };
-        // a NaN or infinity (rare): zero it; bit i of the result: this lane had one among x[8 i' + i]
-        auto drop_bad = [&](float (&x)[U]) -> uint32_t {
-            uint32_t bad = 0;
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                if (abs_bits(x[i]) >= 0x7F800000u) {
-                    bad |= 1u << (i & 7);
-                    x[i] = 0.0f;
-                }
-            }
-            return bad;
-        };
+        const uint32_t c0 = ((lane >> 3) + key) & 3, swap = key & 4;
         for (uint32_t u = warp - kRowsSoftWarps; u < units; u += kRowsConvWarps) {
             const uint32_t j = u / 16, w = u & 7, i = u / 8, sl = i % NR;
+            const bool is_v = (u & 8) != 0;
             if (!warp_wait(&r_full[sl], i / NR, a.err)) break;
             const uint32_t place = (t0 + j) * kRowsKeys + 8 * w;
             // places past the end (never copied) and on bad pages are zeros, hidden from every row
-            uint32_t none = (uint32_t)(rhide[sl] >> (8 * w)) & 0xFFu;
+            uint32_t none = (uint32_t)(rhide[sl] >> (8 * w)) & 0xFFu, bad = 0;
             if (place + 8 > places) none |= places <= place ? 0xFFu : (0xFFu << (places - place)) & 0xFFu;
             const float *src = reinterpret_cast<const float *>(smem + S::off_r + sl * S::slot) + (size_t)8 * w * hd;
             float x[U];
-            if ((u & 8) == 0) {
-                // K: the lane's key is `key`, its chunks of eight dimensions c0, c0 + 4, ..; the
-                // rotation by the key and the swapped halves keep the reads of eight rows and the
-                // writes of one 16-byte column each free of bank conflicts
-                const uint32_t c0 = ((lane >> 3) + key) & 3, swap = key & 4;
+            uint32_t first;  // dimension of the lane's first chunk (V: of its first column)
+            if (!is_v) {
+                // the lane's key is `key`, its chunks of eight dimensions c0, c0 + 4, ..; the rotation by
+                // the key and the swapped halves keep the reads of eight rows and the writes of one
+                // 16-byte column each free of bank conflicts
+                first = 8 * c0;
+                const float *from = src + key * hd + 8 * c0;
 #pragma unroll
                 for (int k = 0; k < HD / 32; ++k) {
-                    const uint32_t d = EXACT || 32 * k + 8 * c0 < hd ? 32 * k + 8 * c0 : 0;
-                    const float4 f = *reinterpret_cast<const float4 *>(src + key * hd + d + swap),
-                                 g = *reinterpret_cast<const float4 *>(src + key * hd + d + (swap ^ 4));
-                    x[8 * k] = f.x, x[8 * k + 1] = f.y, x[8 * k + 2] = f.z, x[8 * k + 3] = f.w;
-                    x[8 * k + 4] = g.x, x[8 * k + 5] = g.y, x[8 * k + 6] = g.z, x[8 * k + 7] = g.w;
+                    const float *at = EXACT || 32 * k + 8 * c0 < hd ? from + 32 * k : from - 8 * c0;
+                    const float4 f = *reinterpret_cast<const float4 *>(at + swap), g = *reinterpret_cast<const float4 *>(at + (swap ^ 4));
+                    x[8 * k] = swap ? g.x : f.x, x[8 * k + 1] = swap ? g.y : f.y, x[8 * k + 2] = swap ? g.z : f.z,
+                    x[8 * k + 3] = swap ? g.w : f.w, x[8 * k + 4] = swap ? f.x : g.x, x[8 * k + 5] = swap ? f.y : g.y,
+                    x[8 * k + 6] = swap ? f.z : g.z, x[8 * k + 7] = swap ? f.w : g.w;
                 }
-                if (none >> key & 1) {
-#pragma unroll
-                    for (int k = 0; k < U; ++k) x[k] = 0.0f;
-                }
-                uint32_t top = largest(x), mark = none << 8;
-                if (top >= 0x7F800000u) {
-                    const uint32_t who = __ballot_sync(0xffffffffu, drop_bad(x) != 0);
-                    mark |= (who | who >> 8 | who >> 16 | who >> 24) & 0xFFu;
-                    top = largest(x);
-                }
-                if (lane == 0) mbar_arrive(&r_empty[sl]);  // every lane's values are in registers
-                const uint32_t st = j % KST;
-                if (j >= KST && !warp_wait(&k_empty[st], j / KST - 1, a.err)) break;
-                const int e = top_exp(top);
-                const float sc = pow2i(kRowsTop - e);
-                // element (key, d): chunk d / 8 of 64 rows
-                uint8_t *dst = smem + S::off_k + st * 2 * S::half + c0 * (kRowsKeys * 16) + w * 128 + key * 16;
-#pragma unroll
-                for (int k = 0; k < HD / 32; ++k) {
-                    if (EXACT || 32 * k + 8 * c0 < hd) {
-                        uint2 h0, h1, l0, l1;
-                        split_f16(x[8 * k] * sc, x[8 * k + 1] * sc, h0.x, l0.x);
-                        split_f16(x[8 * k + 2] * sc, x[8 * k + 3] * sc, h0.y, l0.y);
-                        split_f16(x[8 * k + 4] * sc, x[8 * k + 5] * sc, h1.x, l1.x);
-                        split_f16(x[8 * k + 6] * sc, x[8 * k + 7] * sc, h1.y, l1.y);
-                        *reinterpret_cast<uint4 *>(dst + k * 4 * (kRowsKeys * 16)) =
-                            swap ? make_uint4(h1.x, h1.y, h0.x, h0.y) : make_uint4(h0.x, h0.y, h1.x, h1.y);
-                        *reinterpret_cast<uint4 *>(dst + k * 4 * (kRowsKeys * 16) + S::half) =
-                            swap ? make_uint4(l1.x, l1.y, l0.x, l0.y) : make_uint4(l0.x, l0.y, l1.x, l1.y);
-                    }
-                }
-                if (lane == 0) {
-                    kscale[(j % kRowsMeta) * 8 + w] = pow2i(e - kRowsTop);
-                    kmark[(j % kRowsMeta) * 8 + w] = mark;
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&k_full[st]);
             } else {
-                // V: dimensions lane + 32 k of the eight places
+                // dimensions lane + 32 k of the eight places
+                first = lane;
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
 #pragma unroll
                     for (int k = 0; k < HD / 32; ++k)
                         x[8 * k + c] = src[c * hd + (EXACT || lane + 32 * k < hd ? lane + 32 * k : 0)];
-                if (none != 0) {
+            }
+            if (none != 0) {
 #pragma unroll
-                    for (int k = 0; k < U; ++k)
-                        if (none >> (k & 7) & 1) x[k] = 0.0f;
-                }
-                uint32_t top = largest(x), mark = 0;
-                if (top >= 0x7F800000u) {
-                    mark = __reduce_or_sync(0xffffffffu, drop_bad(x));
-                    top = largest(x);
-                }
-                if (lane == 0) mbar_arrive(&r_empty[sl]);
-                const uint32_t st = j % VST;
-                if (j >= VST && !warp_wait(&v_empty[st], j / VST - 1, a.err)) break;
-                const int e = top_exp(top);
-                const float sc = pow2i(kRowsTop - e);
-                // element (d, place): chunk place / 8 of HD rows
-                uint8_t *dst = smem + S::off_v + st * 2 * S::half + w * (HD * 16) + lane * 16;
+                for (int k = 0; k < U; ++k)
+                    if (none >> (is_v ? k & 7 : key) & 1) x[k] = 0.0f;
+            }
+            uint32_t top = 0;
 #pragma unroll
-                for (int k = 0; k < HD / 32; ++k) {
-                    if (EXACT || lane + 32 * k < hd) {
-                        uint4 h, l;
-                        split_f16(x[8 * k] * sc, x[8 * k + 1] * sc, h.x, l.x);
-                        split_f16(x[8 * k + 2] * sc, x[8 * k + 3] * sc, h.y, l.y);
-                        split_f16(x[8 * k + 4] * sc, x[8 * k + 5] * sc, h.z, l.z);
-                        split_f16(x[8 * k + 6] * sc, x[8 * k + 7] * sc, h.w, l.w);
-                        *reinterpret_cast<uint4 *>(dst + k * 512) = h;
-                        *reinterpret_cast<uint4 *>(dst + k * 512 + S::half) = l;
+            for (int k = 0; k < U; k += 2) top = max(top, max(abs_bits(x[k]), abs_bits(x[k + 1])));
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (top >= 0x7F800000u) {  // a NaN or infinity: zero it, mark its place
+                top = 0;
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    if (abs_bits(x[k]) >= 0x7F800000u) {
+                        bad |= 1u << (is_v ? k & 7 : key);
+                        x[k] = 0.0f;
                     }
+                    top = max(top, abs_bits(x[k]));
                 }
-                if (lane == 0) {
-                    vexp[st * 8 + w] = e;
-                    vmark[st * 8 + w] = mark;
+                top = __reduce_max_sync(0xffffffffu, top);
+                bad = __reduce_or_sync(0xffffffffu, bad);
+            }
+            if (lane == 0) mbar_arrive(&r_empty[sl]);  // every lane's values are in registers
+            const uint32_t st = is_v ? j % VST : j % KST, pass = is_v ? j / VST : j / KST;
+            if (pass > 0 && !warp_wait((is_v ? v_empty : k_empty) + st, pass - 1, a.err)) break;
+            const int e = top_exp(top);
+            const float sc = pow2i(kRowsTop - e);
+            const uint64_t sc2 = pair(sc, sc);
+            // element (key, d) of K: chunk d / 8 of 64 rows; (d, place) of V: chunk place / 8 of HD rows
+            uint8_t *dst = smem + (is_v ? S::off_v + st * 2 * S::half + w * (HD * 16) + lane * 16
+                                        : S::off_k + st * 2 * S::half + c0 * (kRowsKeys * 16) + w * 128 + key * 16);
+            const uint32_t step = is_v ? 32 * 16 : 4 * (kRowsKeys * 16);
+#pragma unroll
+            for (uint32_t k = 0; k < HD / 32; ++k) {
+                if (EXACT || first + 32 * k < hd) {
+                    uint4 h, l;
+                    split_scaled(x[8 * k], x[8 * k + 1], sc2, h.x, l.x);
+                    split_scaled(x[8 * k + 2], x[8 * k + 3], sc2, h.y, l.y);
+                    split_scaled(x[8 * k + 4], x[8 * k + 5], sc2, h.z, l.z);
+                    split_scaled(x[8 * k + 6], x[8 * k + 7], sc2, h.w, l.w);
+                    *reinterpret_cast<uint4 *>(dst + k * step) = h;
+                    *reinterpret_cast<uint4 *>(dst + k * step + S::half) = l;
                 }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&v_full[st]);
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                (is_v ? vmeta + st * 8 : kmeta + (j % kRowsMeta) * 8)[w] = unit_meta(e, none, bad);
+                mbar_arrive((is_v ? v_full : k_full) + st);
             }
         }
     } else if (warp == kRowsMmaWarp) {
@@ -427,43 +434,47 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
         if (lane == 0) {
             const uint32_t id_s = umma_idesc_f16(kRowsM, kRowsKeys), id_o = umma_idesc_f16(kRowsM, hd);
             const uint32_t kb = smem_u32(smem + S::off_k), vb = smem_u32(smem + S::off_v);
+            // S of tile js and O of tile jo, whichever has its operands: K of the next tile
+            // and P of this one are ready in either order
             bool ok = mbar_wait_bounded(q_full, 0, a.err);
-            for (uint32_t j = 0; ok && j <= nt; ++j) {
-                if (j < nt) {  // S of tile j
-                    const uint32_t st = j % KST;
-                    ok = mbar_wait_bounded(&k_full[st], (j / KST) & 1, a.err) &&
-                         (j == 0 || mbar_wait_bounded(s_empty, (j - 1) & 1, a.err));
-                    if (!ok) break;
+            uint32_t js = 0, jo = 0, polls = 0;
+            while (ok && jo < nt) {
+                const uint32_t ks = js % KST, vs = jo % VST, ob = jo & 1;
+                if (js < nt && mbar_try_wait(&k_full[ks], (js / KST) & 1) && (js == 0 || mbar_try_wait(s_empty, (js - 1) & 1))) {
                     tc_fence_after();
-                    const uint32_t kt = kb + st * 2 * S::half;
-#pragma unroll 4
-                    for (uint32_t kk = 0; kk < hd / 16; ++kk) {
-                        const uint64_t kh = umma_desc(kt + kk * 2 * (kRowsKeys * 16), kRowsKeys * 16, 128);
-                        const uint64_t kl = umma_desc(kt + S::half + kk * 2 * (kRowsKeys * 16), kRowsKeys * 16, 128);
+                    const uint32_t kt = kb + ks * 2 * S::half;
+                    // (a descriptor's address field counts 16 bytes)
+                    uint64_t kh = umma_desc(kt, kRowsKeys * 16, 128), kl = umma_desc(kt + S::half, kRowsKeys * 16, 128);
+#pragma unroll 1
+                    for (uint32_t kk = 0; kk < hd / 16; ++kk, kh += 2 * kRowsKeys, kl += 2 * kRowsKeys) {
                         umma_16_ts(tm_s, tm_q + kk * 8, kh, id_s, kk > 0);
                         umma_16_ts(tm_s, tm_q + HD / 2 + kk * 8, kh, id_s, 1);
                         umma_16_ts(tm_s, tm_q + kk * 8, kl, id_s, 1);
                     }
                     umma_commit(s_full);
-                    umma_commit(&k_empty[st]);
+                    umma_commit(&k_empty[ks]);
+                    ++js;
+                    polls = 0;
                 }
-                if (j > 0) {  // O of tile j - 1
-                    const uint32_t i = j - 1, st = i % VST, ob = i & 1;
-                    ok = mbar_wait_bounded(p_full, i & 1, a.err) && mbar_wait_bounded(&v_full[st], (i / VST) & 1, a.err) &&
-                         (i < 2 || mbar_wait_bounded(&o_empty[ob], (i / 2 - 1) & 1, a.err));
-                    if (!ok) break;
+                if (jo < js && mbar_try_wait(p_full, jo & 1) && mbar_try_wait(&v_full[vs], (jo / VST) & 1) &&
+                    (jo < 2 || mbar_try_wait(&o_empty[ob], (jo / 2 - 1) & 1))) {
                     tc_fence_after();
-                    const uint32_t d = tm_o + ob * HD, vt = vb + st * 2 * S::half;
-#pragma unroll
-                    for (uint32_t kk = 0; kk < kRowsKeys / 16; ++kk) {
-                        const uint64_t vh = umma_desc(vt + kk * 2 * (HD * 16), HD * 16, 128);
-                        const uint64_t vl = umma_desc(vt + S::half + kk * 2 * (HD * 16), HD * 16, 128);
+                    const uint32_t d = tm_o + ob * HD, vt = vb + vs * 2 * S::half;
+                    uint64_t vh = umma_desc(vt, HD * 16, 128), vl = umma_desc(vt + S::half, HD * 16, 128);
+#pragma unroll 1
+                    for (uint32_t kk = 0; kk < kRowsKeys / 16; ++kk, vh += 2 * HD, vl += 2 * HD) {
                         umma_16_ts(d, tm_p + kk * 8, vh, id_o, kk > 0);
                         umma_16_ts(d, tm_p + 32 + kk * 8, vh, id_o, 1);
                         umma_16_ts(d, tm_p + kk * 8, vl, id_o, 1);
                     }
                     umma_commit(&o_full[ob]);
-                    umma_commit(&v_empty[st]);
+                    umma_commit(&v_empty[vs]);
+                    ++jo;
+                    polls = 0;
+                }
+                if (++polls > (1u << 22)) {
+                    raise_error(a.err, B2_ERR_TIMEOUT);
+                    ok = false;
                 }
             }
             // everything issued has completed before tensor memory is freed
@@ -512,28 +523,32 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
             }
             const uint64_t mask = mine && a.tree != nullptr ? a.tree[r0 + tok] : 0;
             float m = -INFINITY, l = 0.0f, corr_prev = 0.0f, osc_prev = 0.0f;
-            float acc[HD / 2];
+            uint64_t acc[HD / 4];  // pairs of the half's dimensions
 #pragma unroll
-            for (int i = 0; i < HD / 2; ++i) acc[i] = 0.0f;
+            for (int i = 0; i < HD / 4; ++i) acc[i] = 0;
+            // The two warps of a quarter meet at a named barrier once a tile, so neither may leave
+            // the loop alone: after a wait that gave up both run on without waiting.
+            bool ok = true;
+            auto wait = [&](uint64_t *bar, uint32_t phase) { ok = ok && warp_wait(bar, phase, a.err); };
+            auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + qt) : "memory"); };
             // O of tile i into the sums: acc = acc * corr + O * osc
             auto take_o = [&](uint32_t i) {
                 const uint32_t col = tm_o + lanes + (i & 1) * HD + half * (HD / 2);
                 tc_fence_after();
                 if (!__all_sync(0xffffffffu, corr_prev == 1.0f || !mine)) {
+                    const uint64_t c2 = pair(corr_prev, corr_prev);
 #pragma unroll
-                    for (int k = 0; k < HD / 2; ++k) acc[k] *= corr_prev;
+                    for (int k = 0; k < HD / 4; ++k) acc[k] = mul2(acc[k], c2);
                 }
+                const uint64_t o2 = pair(osc_prev, osc_prev);
 #pragma unroll
                 for (int c = 0; c < HD / 2; c += 32) {
-                    uint32_t v[16], w[16];
-                    tmem_ld16_nowait(col + c, v);
-                    tmem_ld16_nowait(col + c + 16, w);
+                    uint32_t v[32];
+                    tmem_ld32(col + c, v);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        acc[c + k] = fmaf(__uint_as_float(v[k]), osc_prev, acc[c + k]);
-                        acc[c + 16 + k] = fmaf(__uint_as_float(w[k]), osc_prev, acc[c + 16 + k]);
-                    }
+                    for (int k = 0; k < 16; ++k)
+                        acc[c / 2 + k] = fma2(pair(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), o2, acc[c / 2 + k]);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -559,91 +574,80 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 if (key0 + 32 > places) vis &= places <= key0 ? 0 : (1u << (places - key0)) - 1;
                 return vis;
             };
-            bool ok = true;
             for (uint32_t j = 0; j < nt; ++j) {
-                const uint32_t mt = j % kRowsMeta, vt = j % VST;
-                ok = warp_wait(s_full, j, a.err);
-                if (!ok) break;
+                const uint32_t mt = j % kRowsMeta, vt = j % VST, key0 = (t0 + j) * kRowsKeys + half * 32;
+                wait(s_full, j);
                 tc_fence_after();
-                float s[32], top = -INFINITY;
-                // the other half's scores, for the maximum alone, then this half's
-                float ks0 = 0.0f;
+                uint32_t raw[32];
+                tmem_ld32(tm_s + lanes + half * 32, raw);
+                const uint4 km = *reinterpret_cast<const uint4 *>(kmeta + mt * 8 + half * 4);
+                tmem_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_empty);
+                float s[32];
 #pragma unroll
-                for (int o = 0; o < 2; ++o) {
-                    const uint32_t hh = o == 0 ? half ^ 1 : half;
-                    const float4 ks = *reinterpret_cast<const float4 *>(kscale + mt * 8 + hh * 4);
-                    const uint4 km = *reinterpret_cast<const uint4 *>(kmark + mt * 8 + hh * 4);
-                    uint32_t u[16], v[16];
-                    tmem_ld16_nowait(tm_s + lanes + hh * 32, u);
-                    tmem_ld16_nowait(tm_s + lanes + hh * 32 + 16, v);
-                    tmem_wait_ld();
-                    if (o == 1) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(s_empty);
+                for (int k = 0; k < 32; ++k) s[k] = __uint_as_float(raw[k]);
+                int ks = meta_exp(km.x);
+                uint32_t vis = key0 + 32 > ctx ? visible(key0) : 0xFFFFFFFFu;
+                if (!meta_plain(km)) {  // units of different scale, places hidden or not finite
+                    const int eu[4] = {ks, meta_exp(km.y), meta_exp(km.z), meta_exp(km.w)};
+                    ks = max(max(eu[0], eu[1]), max(eu[2], eu[3]));
+                    const uint32_t bad = meta_bytes(km, 0);
+                    vis &= ~meta_bytes(km, 8);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        s[k] *= pow2i(max(eu[k / 8] - ks, -126));
+                        if (bad >> k & 1) s[k] = NAN;
                     }
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        s[k] = __uint_as_float(u[k]);
-                        s[16 + k] = __uint_as_float(v[k]);
-                    }
-                    ks0 = fmaxf(fmaxf(ks.x, ks.y), fmaxf(ks.z, ks.w));
-                    if (ks.x != ks0 || ks.y != ks0 || ks.z != ks0 || ks.w != ks0) {  // units of different scale: to the largest
-                        const float f[4] = {ks.x / ks0, ks.y / ks0, ks.z / ks0, ks.w / ks0};
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) s[k] *= f[k / 8];
-                    }
-                    uint32_t vis = visible((t0 + j) * kRowsKeys + hh * 32);
-                    if ((km.x | km.y | km.z | km.w) != 0) {
-                        const uint32_t bad = (km.x & 0xFF) | (km.y & 0xFF) << 8 | (km.z & 0xFF) << 16 | (km.w & 0xFF) << 24;
-                        vis &= ~((km.x >> 8) | (km.y >> 8) << 8 | (km.z >> 8) << 16 | (km.w >> 8) << 24);
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (bad >> k & 1) s[k] = NAN;
-                    }
-                    if (vis != 0xFFFFFFFFu) {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (!(vis >> k & 1)) s[k] = -INFINITY;
-                    }
-                    float t = s[0];
-#pragma unroll
-                    for (int k = 1; k < 32; ++k) t = fmaxf(t, s[k]);
-                    top = fmaxf(top, t * ks0);
                 }
-                const float m_new = fmaxf(m, top * cq);
+                if (vis != 0xFFFFFFFFu) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k)
+                        if (!(vis >> k & 1)) s[k] = -INFINITY;
+                }
+                float top = fmaxf(s[0], s[1]);
+#pragma unroll
+                for (int k = 2; k < 32; k += 2) top = fmaxf(top, fmaxf(s[k], s[k + 1]));
+                const float cqk = cq * pow2i(ks - kRowsTop);
+                // the row's maximum over both halves
+                float *x = xmax + (j & 1) * 2 * kRowsM;
+                x[half * kRowsM + r] = top * cqk;
+                meet();
+                const float m_new = fmaxf(m, fmaxf(top * cqk, x[(half ^ 1) * kRowsM + r]));
                 const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-                const float corr = ex2(m - m_use), shift = kRowsP - m_use, cqk = cq * ks0;
-                float sum = 0.0f;
-#pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                    s[k] = ex2(fmaf(s[k], cqk, shift));
-                    sum += s[k];
-                }
-                l = fmaf(l, corr, sum);
+                const float corr = ex2(m - m_use);
                 m = m_new;
-                ok = warp_wait(&v_full[vt], j / VST, a.err);
-                if (!ok) break;
-                const int4 e0 = *reinterpret_cast<const int4 *>(vexp + vt * 8), e1 = *reinterpret_cast<const int4 *>(vexp + vt * 8 + 4);
-                const uint4 vm = *reinterpret_cast<const uint4 *>(vmark + vt * 8 + half * 4);
-                const int emax = max(max(max(e0.x, e0.y), max(e0.z, e0.w)), max(max(e1.x, e1.y), max(e1.z, e1.w)));
-                const int4 eh = half ? e1 : e0;
-                if ((eh.x & eh.y & eh.z & eh.w) != emax || (eh.x | eh.y | eh.z | eh.w) != emax) {  // not all the tile's largest
-                    const int eg[4] = {eh.x, eh.y, eh.z, eh.w};
+                const uint64_t cq2 = pair(cqk, cqk), sh2 = pair(kRowsP - m_use, kRowsP - m_use);
+                uint64_t sum = 0;
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) s[k] *= pow2i(max(eg[k / 8] - emax, -126));
+                for (int k = 0; k < 32; k += 2) {
+                    float y, z;
+                    unpair(fma2(pair(s[k], s[k + 1]), cq2, sh2), y, z);
+                    s[k] = ex2(y);
+                    s[k + 1] = ex2(z);
+                    sum = add2(sum, pair(s[k], s[k + 1]));
                 }
-                if ((vm.x | vm.y | vm.z | vm.w) != 0) {  // a NaN or infinity in V reaches the rows that see its place
-                    const uint32_t bad = (vm.x & 0xFF) | (vm.y & 0xFF) << 8 | (vm.z & 0xFF) << 16 | (vm.w & 0xFF) << 24;
-                    const uint32_t hit = bad & visible((t0 + j) * kRowsKeys + half * 32);
-                    if (hit != 0) l = NAN;
+                float sy, sz;
+                unpair(sum, sy, sz);
+                l = fmaf(l, corr, sy + sz);
+                wait(&v_full[vt], j / VST);
+                const uint4 va = *reinterpret_cast<const uint4 *>(vmeta + vt * 8), vb = *reinterpret_cast<const uint4 *>(vmeta + vt * 8 + 4);
+                int emax = meta_exp(va.x);
+                if (!meta_plain(va) || !meta_plain(vb) || va.x != vb.x) {  // units of different scale, or a NaN or infinity in V
+                    emax = max(max(max(emax, meta_exp(va.y)), max(meta_exp(va.z), meta_exp(va.w))),
+                               max(max(meta_exp(vb.x), meta_exp(vb.y)), max(meta_exp(vb.z), meta_exp(vb.w))));
+                    const uint4 vh = half ? vb : va;
+                    const int eu[4] = {meta_exp(vh.x), meta_exp(vh.y), meta_exp(vh.z), meta_exp(vh.w)};
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) s[k] *= pow2i(max(eu[k / 8] - emax, -126));
+                    if ((meta_bytes(vh, 0) & visible(key0)) != 0) l = NAN;
                 }
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) split_f16(s[2 * k], s[2 * k + 1], hi[k], lo[k]);
                 if (j > 0) {
-                    ok = warp_wait(&o_full[(j - 1) & 1], (j - 1) / 2, a.err);  // P is free, and O of tile j - 1 is there
-                    if (!ok) break;
+                    wait(&o_full[(j - 1) & 1], (j - 1) / 2);  // P is free, and O of tile j - 1 is there
                     tc_fence_after();
                 }
                 tmem_st16(tm_p + lanes + half * 16, hi);
@@ -656,16 +660,19 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 corr_prev = corr;
                 osc_prev = pow2i(emax - kRowsTop - (int)kRowsP);
             }
-            if (ok) ok = warp_wait(&o_full[(nt - 1) & 1], (nt - 1) / 2, a.err);
-            if (ok) {
-                take_o(nt - 1);
-                // the row's sum: both halves', in one order
-                xsum[half * kRowsM + r] = l;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&xbar[qt]);
-                ok = warp_wait(&xbar[qt], 0, a.err);
-                l = xsum[r] + xsum[kRowsM + r];
-            }
+            wait(&o_full[(nt - 1) & 1], (nt - 1) / 2);
+            take_o(nt - 1);
+            // the row's sum: both halves', in one order
+            float *x = xmax + (nt & 1) * 2 * kRowsM;
+            x[half * kRowsM + r] = l;
+            meet();
+            l = x[r] + x[kRowsM + r];
+            auto acc4 = [&](int c) {
+                float4 f;
+                unpair(acc[c / 2], f.x, f.y);
+                unpair(acc[c / 2 + 1], f.z, f.w);
+                return f;
+            };
             if (ok && mine) {
                 // the weights carry 2^12, the sums of O do not
                 const float lw = l * pow2i(-(int)kRowsP);
@@ -677,7 +684,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
 #pragma unroll
                     for (int c = 0; c < HD / 2; c += 4)
                         if (half * (HD / 2) + c < hd)
-                            *reinterpret_cast<float4 *>(dst + half * (HD / 2) + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+                            *reinterpret_cast<float4 *>(dst + half * (HD / 2) + c) = acc4(c);
                 } else {
                     const float inv = lw > 0.0f ? 1.0f / lw : lw == 0.0f ? 0.0f : lw;  // NaN stays
                     if (lw != lw && half == 0) raise_error(a.err, B2_ERR_NONFINITE);
@@ -686,7 +693,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                     for (int c = 0; c < HD / 2; c += 4)
                         if (half * (HD / 2) + c < hd)
                             *reinterpret_cast<float4 *>(dst + half * (HD / 2) + c) =
-                                make_float4(acc[c] * inv, acc[c + 1] * inv, acc[c + 2] * inv, acc[c + 3] * inv);
+                                make_float4(acc4(c).x * inv, acc4(c).y * inv, acc4(c).z * inv, acc4(c).w * inv);
                 }
             }
         }
