@@ -9,12 +9,12 @@
 // Work split. The rows of an item times the query heads of one KV head are the
 // rows r = token * group + head of a matrix; CTA (split, KV head and block of
 // 128 such rows, item) takes a contiguous range of the places in tiles of 64, so
-// K and V are read once per 128 rows. 16 warps (128 registers a thread):
-//   warp 15       streams K and V (f32) into a ring of tiles with bulk copies, a
+// K and V are read once per 128 rows. Five warpgroups:
+//   warp 17       streams K and V (f32) into a ring of tiles with bulk copies, a
 //                 run of places on one page each;
-//   warps 8..13   convert: units of eight places' K or V from the ring into matrix
-//                 operands;
-//   warp 14       one thread issues the tcgen05 MMAs: S = Q K^T of tile j + 1
+//   warps 8..15   convert 16 places each of every tile's K (8..11) or V (12..15) from
+//                 the ring into matrix operands;
+//   warp 16       one thread issues the tcgen05 MMAs: S = Q K^T of tile j + 1
 //                 before O = P V of tile j; Q, P, S and O live in tensor memory
 //                 (O in two buffers), only K and V are read from shared memory;
 //   warps 0..7    two per 32 rows: a thread holds one row and 32 of a tile's 64
@@ -31,9 +31,10 @@
 // hi hi + lo hi + hi lo with f32 accumulation; what is dropped is below 2^-22.
 // f16 rather than bf16 pairs (2^-16) because the scale takes care of the range:
 // a row of q, eight places' K and eight places' V have a power of two each that
-// brings their largest magnitude to [2^8, 2^12), so an element 2^-17 of the
-// largest still keeps 16 bits. (The exponents are multiples of four, so that
-// neighbours mostly share one and the factors below drop out.) K's scale goes
+// brings their largest magnitude to [1, 16), so an element 2^-9 of the largest
+// still keeps 16 bits, and what a smaller one loses is below 2^-25 of the largest.
+// (The exponents are multiples of four, so that neighbours mostly share one, and
+// mostly have none to apply.) K's scale goes
 // into the scores, V's into P relative to the tile's largest, and the tile's
 // into its O when it is summed. The softmax statistics and the weighted sums are
 // f32.
@@ -55,18 +56,23 @@ namespace b2 {
 constexpr uint32_t kRowsM = 128;        // (token, query head) rows of a CTA
 constexpr uint32_t kRowsKeys = 64;      // places of a tile
 constexpr int kRowsSoftWarps = 8;
-constexpr int kRowsConvWarps = 6;
+constexpr int kRowsConvWarps = 8;
 constexpr uint32_t kRowsMmaWarp = kRowsSoftWarps + kRowsConvWarps, kRowsCopyWarp = kRowsMmaWarp + 1;
-constexpr int kRowsThreads = 32 * (kRowsSoftWarps + kRowsConvWarps + 2);
+constexpr int kRowsThreads = 32 * (kRowsSoftWarps + kRowsConvWarps + 4);  // whole warpgroups: two warps idle
+// Registers a thread of the softmax warpgroups (two), the converting ones (two) and
+// the last one; the launch gives every thread 96 (five warps per scheduler).
+constexpr int kRowsSoftRegs = 136, kRowsConvRegs = 80, kRowsLastRegs = 40;
+static_assert(kRowsThreads == 640 && 256 * kRowsSoftRegs + 256 * kRowsConvRegs + 128 * kRowsLastRegs <= 640 * 96, "register split");
+constexpr uint32_t kRowsUnit = 16;      // places a converting warp takes of a tile
 constexpr uint32_t kRowsMeta = 8;       // ring of per-tile scales: more than the tiles between converting and softmax
 constexpr uint32_t kRowsMaxSplits = 64;
-constexpr int kRowsTop = 8;             // operands are scaled to [2^kRowsTop, 2^(kRowsTop + 4))
+constexpr int kRowsTop = 0;             // operands are scaled to [2^kRowsTop, 2^(kRowsTop + 4))
 constexpr float kRowsP = 12.0f;         // P is scaled by 2^12
 
 template <int HD>
 struct RowsSmem {
-    static constexpr uint32_t k_stages = HD == 128 ? 1 : 2, v_stages = 2;
-    static constexpr uint32_t slots = HD == 128 ? 4 : 6;           // ring of f32 tiles, K and V in turn
+    static constexpr uint32_t k_stages = 2, v_stages = 2;
+    static constexpr uint32_t slots = HD == 128 ? 3 : 6;           // ring of f32 tiles, K and V in turn
     static constexpr uint32_t slot = kRowsKeys * HD * 4;
     static constexpr uint32_t half = kRowsKeys * HD * 2;           // hi or lo of an operand
     static constexpr uint32_t off_k = 0;
@@ -138,6 +144,16 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
+// The same with hi cut off instead of rounded (a mask instead of a conversion
+// back): 21 bits together, for the weights, whose lo is then never negative.
+__device__ __forceinline__ void cut_f16(float a, float b, uint32_t &hi, uint32_t &lo)
+{
+    const float ha = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u), hb = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
+    const __half2 h = __floats2half2_rn(ha, hb), l = __floats2half2_rn(a - ha, b - hb);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
 // What the softmax needs to know of a unit: exponent, places hidden from every
 // row, places with a NaN or infinity.
 __device__ __forceinline__ uint32_t unit_meta(int e, uint32_t hidden, uint32_t bad) { return (uint32_t)(e + 128) << 16 | hidden << 8 | bad; }
@@ -177,12 +193,12 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
     return r;
 }
 
-// The same of two values scaled by the pair sc2.
-__device__ __forceinline__ void split_scaled(float a, float b, uint64_t sc2, uint32_t &hi, uint32_t &lo)
+// Largest of three, NaN if one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c)
 {
-    float x, y;
-    unpair(mul2(pair(a, b), sc2), x, y);
-    split_f16(x, y, hi, lo);
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
@@ -252,14 +268,14 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < NR; ++i) {
             mbar_init(&r_full[i], 1);
-            mbar_init(&r_empty[i], kRowsKeys / 8);
+            mbar_init(&r_empty[i], kRowsKeys / kRowsUnit);
         }
         for (uint32_t i = 0; i < KST; ++i) {
-            mbar_init(&k_full[i], kRowsKeys / 8);
+            mbar_init(&k_full[i], kRowsKeys / kRowsUnit);
             mbar_init(&k_empty[i], 1);
         }
         for (uint32_t i = 0; i < VST; ++i) {
-            mbar_init(&v_full[i], kRowsKeys / 8);
+            mbar_init(&v_full[i], kRowsKeys / kRowsUnit);
             mbar_init(&v_empty[i], 1);
         }
         mbar_init(s_full, 1);
@@ -281,208 +297,221 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
     // columns: S 64 | P hi 32, lo 32 | Q hi HD / 2, lo HD / 2 | O from 256, two buffers of HD
     const uint32_t tm_s = tmem, tm_p = tmem + 64, tm_q = tmem + 128, tm_o = tmem + 256;
 
-    if (warp == kRowsCopyWarp) {
-        // ---- K and V tiles into the ring: lane l looks after places l and l + 32 ----
-        const int32_t *table = a.kv.page_table + (size_t)item * a.kv.pages_per_seq;
-        const uint32_t pt = a.kv.page_tokens, rowb = hd * sizeof(float);
-        const uint64_t pol = l2_evict_first_policy();
-        int fault = 0;
-        auto page_of = [&](uint32_t t, uint32_t h) -> int32_t {
-            const uint32_t at = (t0 + t) * kRowsKeys + lane + 32 * h;
-            return t < nt && at < places ? table[at / pt] : 0;
-        };
-        int32_t page[2] = {page_of(0, 0), page_of(0, 1)};
-        uint32_t filled = 0;
-        bool ok = true;
-        for (uint32_t j = 0; ok && j < nt; ++j) {
-            size_t row[2];
-            uint32_t run[2], bytes = 0, bad[2];
+    if (warp >= kRowsMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRowsLastRegs));
+        if (warp == kRowsCopyWarp) {
+            // ---- K and V tiles into the ring: lane l looks after places l and l + 32 ----
+            const int32_t *table = a.kv.page_table + (size_t)item * a.kv.pages_per_seq;
+            const uint32_t pt = a.kv.page_tokens, rowb = hd * sizeof(float);
+            const uint64_t pol = l2_evict_first_policy();
+            int fault = 0;
+            auto page_of = [&](uint32_t t, uint32_t h) -> int32_t {
+                const uint32_t at = (t0 + t) * kRowsKeys + lane + 32 * h;
+                return t < nt && at < places ? table[at / pt] : 0;
+            };
+            int32_t page[2] = {page_of(0, 0), page_of(0, 1)};
+            uint32_t filled = 0;
+            bool ok = true;
+            for (uint32_t j = 0; ok && j < nt; ++j) {
+                size_t row[2];
+                uint32_t run[2], bytes = 0, bad[2];
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-                const uint32_t k = lane + 32 * h, at = (t0 + j) * kRowsKeys + k, off = at % pt;
-                const bool in = at < places;
-                const bool wrong = in && (page[h] < 0 || (a.pool_pages != 0 && (uint32_t)page[h] >= a.pool_pages));
-                bad[h] = __ballot_sync(0xffffffffu, wrong);
-                if (wrong) fault = B2_ERR_POSITION;
-                // a run: the tile's places on one page, copied by its first place's lane
-                const bool first = in && !wrong && (k == 0 || off == 0);
-                run[h] = first ? min(min(kRowsKeys - k, pt - off), places - at) : 0;
-                row[h] = (((size_t)(uint32_t)page[h] * a.n_kv_heads + kvh) * pt + off) * hd;
-                bytes += run[h] * rowb;
-                page[h] = page_of(j + 1, h);
-            }
-            bytes = __reduce_add_sync(0xffffffffu, bytes);
-#pragma unroll
-            for (uint32_t op = 0; op < 2 && ok; ++op) {
-                const uint32_t i = 2 * j + op, sl = i % NR;
-                if (i >= NR) ok = warp_wait(&r_empty[sl], i / NR - 1, a.err);
-                if (!ok) break;
-                if (lane == 0) {
-                    rhide[sl] = (uint64_t)bad[1] << 32 | bad[0];
-                    mbar_arrive_expect_tx(&r_full[sl], bytes);
+                for (uint32_t h = 0; h < 2; ++h) {
+                    const uint32_t k = lane + 32 * h, at = (t0 + j) * kRowsKeys + k, off = at % pt;
+                    const bool in = at < places;
+                    const bool wrong = in && (page[h] < 0 || (a.pool_pages != 0 && (uint32_t)page[h] >= a.pool_pages));
+                    bad[h] = __ballot_sync(0xffffffffu, wrong);
+                    if (wrong) fault = B2_ERR_POSITION;
+                    // a run: the tile's places on one page, copied by its first place's lane
+                    const bool first = in && !wrong && (k == 0 || off == 0);
+                    run[h] = first ? min(min(kRowsKeys - k, pt - off), places - at) : 0;
+                    row[h] = (((size_t)(uint32_t)page[h] * a.n_kv_heads + kvh) * pt + off) * hd;
+                    bytes += run[h] * rowb;
+                    page[h] = page_of(j + 1, h);
                 }
-                __syncwarp();
-                const float *pool = op == 0 ? a.kv.k_pool : a.kv.v_pool;
+                bytes = __reduce_add_sync(0xffffffffu, bytes);
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h)
-                    if (run[h] != 0)
-                        bulk_g2s_stream(smem + S::off_r + sl * S::slot + (lane + 32 * h) * rowb, pool + row[h], run[h] * rowb,
-                                        &r_full[sl], pol);
-                filled = i + 1;
-            }
-        }
-        // no copy is in flight when the CTA ends, not even after a wait that gave up
-        for (uint32_t i = filled > NR ? filled - NR : 0; i < filled; ++i) warp_wait(&r_full[i % NR], i / NR, a.err);
-        if (fault) raise_error(a.err, fault);
-    } else if (warp >= (uint32_t)kRowsSoftWarps && warp < kRowsMmaWarp) {
-        // ---- ring tiles into operands ----
-        // Units of eight places' K or V, 16 to a tile (K 0..7, V 0..7), dealt to the
-        // warps in turn. K and V differ in how a lane picks its values; the conversion of
-        // its HD / 32 chunks of eight (16 bytes of hi, 16 of lo) is one piece of code for
-        // both: the roles of this kernel run different code side by side, and instruction
-        // fetch is what they run out of first.
-        constexpr int U = HD / 4;  // values a lane holds of a unit
-        const uint32_t units = nt * 16, key = lane & 7;
-        const uint32_t c0 = ((lane >> 3) + key) & 3, swap = key & 4;
-        for (uint32_t u = warp - kRowsSoftWarps; u < units; u += kRowsConvWarps) {
-            const uint32_t j = u / 16, w = u & 7, i = u / 8, sl = i % NR;
-            const bool is_v = (u & 8) != 0;
-            if (!warp_wait(&r_full[sl], i / NR, a.err)) break;
-            const uint32_t place = (t0 + j) * kRowsKeys + 8 * w;
-            // places past the end (never copied) and on bad pages are zeros, hidden from every row
-            uint32_t none = (uint32_t)(rhide[sl] >> (8 * w)) & 0xFFu, bad = 0;
-            if (place + 8 > places) none |= places <= place ? 0xFFu : (0xFFu << (places - place)) & 0xFFu;
-            const float *src = reinterpret_cast<const float *>(smem + S::off_r + sl * S::slot) + (size_t)8 * w * hd;
-            float x[U];
-            uint32_t first;  // dimension of the lane's first chunk (V: of its first column)
-            if (!is_v) {
-                // the lane's key is `key`, its chunks of eight dimensions c0, c0 + 4, ..; the rotation by
-                // the key and the swapped halves keep the reads of eight rows and the writes of one
-                // 16-byte column each free of bank conflicts
-                first = 8 * c0;
-                const float *from = src + key * hd + 8 * c0;
-#pragma unroll
-                for (int k = 0; k < HD / 32; ++k) {
-                    const float *at = EXACT || 32 * k + 8 * c0 < hd ? from + 32 * k : from - 8 * c0;
-                    const float4 f = *reinterpret_cast<const float4 *>(at + swap), g = *reinterpret_cast<const float4 *>(at + (swap ^ 4));
-                    x[8 * k] = swap ? g.x : f.x, x[8 * k + 1] = swap ? g.y : f.y, x[8 * k + 2] = swap ? g.z : f.z,
-                    x[8 * k + 3] = swap ? g.w : f.w, x[8 * k + 4] = swap ? f.x : g.x, x[8 * k + 5] = swap ? f.y : g.y,
-                    x[8 * k + 6] = swap ? f.z : g.z, x[8 * k + 7] = swap ? f.w : g.w;
-                }
-            } else {
-                // dimensions lane + 32 k of the eight places
-                first = lane;
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-#pragma unroll
-                    for (int k = 0; k < HD / 32; ++k)
-                        x[8 * k + c] = src[c * hd + (EXACT || lane + 32 * k < hd ? lane + 32 * k : 0)];
-            }
-            if (none != 0) {
-#pragma unroll
-                for (int k = 0; k < U; ++k)
-                    if (none >> (is_v ? k & 7 : key) & 1) x[k] = 0.0f;
-            }
-            uint32_t top = 0;
-#pragma unroll
-            for (int k = 0; k < U; k += 2) top = max(top, max(abs_bits(x[k]), abs_bits(x[k + 1])));
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (top >= 0x7F800000u) {  // a NaN or infinity: zero it, mark its place
-                top = 0;
-#pragma unroll
-                for (int k = 0; k < U; ++k) {
-                    if (abs_bits(x[k]) >= 0x7F800000u) {
-                        bad |= 1u << (is_v ? k & 7 : key);
-                        x[k] = 0.0f;
+                for (uint32_t op = 0; op < 2 && ok; ++op) {
+                    const uint32_t i = 2 * j + op, sl = i % NR;
+                    if (i >= NR) ok = warp_wait(&r_empty[sl], i / NR - 1, a.err);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        rhide[sl] = (uint64_t)bad[1] << 32 | bad[0];
+                        mbar_arrive_expect_tx(&r_full[sl], bytes);
                     }
-                    top = max(top, abs_bits(x[k]));
-                }
-                top = __reduce_max_sync(0xffffffffu, top);
-                bad = __reduce_or_sync(0xffffffffu, bad);
-            }
-            if (lane == 0) mbar_arrive(&r_empty[sl]);  // every lane's values are in registers
-            const uint32_t st = is_v ? j % VST : j % KST, pass = is_v ? j / VST : j / KST;
-            if (pass > 0 && !warp_wait((is_v ? v_empty : k_empty) + st, pass - 1, a.err)) break;
-            const int e = top_exp(top);
-            const float sc = pow2i(kRowsTop - e);
-            const uint64_t sc2 = pair(sc, sc);
-            // element (key, d) of K: chunk d / 8 of 64 rows; (d, place) of V: chunk place / 8 of HD rows
-            uint8_t *dst = smem + (is_v ? S::off_v + st * 2 * S::half + w * (HD * 16) + lane * 16
-                                        : S::off_k + st * 2 * S::half + c0 * (kRowsKeys * 16) + w * 128 + key * 16);
-            const uint32_t step = is_v ? 32 * 16 : 4 * (kRowsKeys * 16);
+                    __syncwarp();
+                    const float *pool = op == 0 ? a.kv.k_pool : a.kv.v_pool;
 #pragma unroll
-            for (uint32_t k = 0; k < HD / 32; ++k) {
-                if (EXACT || first + 32 * k < hd) {
-                    uint4 h, l;
-                    split_scaled(x[8 * k], x[8 * k + 1], sc2, h.x, l.x);
-                    split_scaled(x[8 * k + 2], x[8 * k + 3], sc2, h.y, l.y);
-                    split_scaled(x[8 * k + 4], x[8 * k + 5], sc2, h.z, l.z);
-                    split_scaled(x[8 * k + 6], x[8 * k + 7], sc2, h.w, l.w);
-                    *reinterpret_cast<uint4 *>(dst + k * step) = h;
-                    *reinterpret_cast<uint4 *>(dst + k * step + S::half) = l;
+                    for (uint32_t h = 0; h < 2; ++h)
+                        if (run[h] != 0)
+                            bulk_g2s_stream(smem + S::off_r + sl * S::slot + (lane + 32 * h) * rowb, pool + row[h], run[h] * rowb,
+                                            &r_full[sl], pol);
+                    filled = i + 1;
                 }
+            }
+            // no copy is in flight when the CTA ends, not even after a wait that gave up
+            for (uint32_t i = filled > NR ? filled - NR : 0; i < filled; ++i) warp_wait(&r_full[i % NR], i / NR, a.err);
+            if (fault) raise_error(a.err, fault);
+        } else if (warp == kRowsMmaWarp) {
+            // ---- MMA issue ----
+            if (lane == 0) {
+                const uint32_t id_s = umma_idesc_f16(kRowsM, kRowsKeys), id_o = umma_idesc_f16(kRowsM, hd);
+                const uint32_t kb = smem_u32(smem + S::off_k), vb = smem_u32(smem + S::off_v);
+                // S of tile js and O of tile jo, whichever has its operands: K of the next tile
+                // and P of this one are ready in either order
+                bool ok = mbar_wait_bounded(q_full, 0, a.err);
+                uint32_t js = 0, jo = 0, polls = 0;
+                while (ok && jo < nt) {
+                    const uint32_t ks = js % KST, vs = jo % VST, ob = jo & 1;
+                    if (js < nt && mbar_try_wait(&k_full[ks], (js / KST) & 1) && (js == 0 || mbar_try_wait(s_empty, (js - 1) & 1))) {
+                        tc_fence_after();
+                        const uint32_t kt = kb + ks * 2 * S::half;
+                        // (a descriptor's address field counts 16 bytes)
+                        uint64_t kh = umma_desc(kt, kRowsKeys * 16, 128), kl = umma_desc(kt + S::half, kRowsKeys * 16, 128);
+#pragma unroll 1
+                        for (uint32_t kk = 0; kk < hd / 16; ++kk, kh += 2 * kRowsKeys, kl += 2 * kRowsKeys) {
+                            umma_16_ts(tm_s, tm_q + kk * 8, kh, id_s, kk > 0);
+                            umma_16_ts(tm_s, tm_q + HD / 2 + kk * 8, kh, id_s, 1);
+                            umma_16_ts(tm_s, tm_q + kk * 8, kl, id_s, 1);
+                        }
+                        umma_commit(s_full);
+                        umma_commit(&k_empty[ks]);
+                        ++js;
+                        polls = 0;
+                    }
+                    if (jo < js && mbar_try_wait(p_full, jo & 1) && mbar_try_wait(&v_full[vs], (jo / VST) & 1) &&
+                        (jo < 2 || mbar_try_wait(&o_empty[ob], (jo / 2 - 1) & 1))) {
+                        tc_fence_after();
+                        const uint32_t d = tm_o + ob * HD, vt = vb + vs * 2 * S::half;
+                        uint64_t vh = umma_desc(vt, HD * 16, 128), vl = umma_desc(vt + S::half, HD * 16, 128);
+#pragma unroll 1
+                        for (uint32_t kk = 0; kk < kRowsKeys / 16; ++kk, vh += 2 * HD, vl += 2 * HD) {
+                            umma_16_ts(d, tm_p + kk * 8, vh, id_o, kk > 0);
+                            umma_16_ts(d, tm_p + 32 + kk * 8, vh, id_o, 1);
+                            umma_16_ts(d, tm_p + kk * 8, vl, id_o, 1);
+                        }
+                        umma_commit(&o_full[ob]);
+                        umma_commit(&v_empty[vs]);
+                        ++jo;
+                        polls = 0;
+                    }
+                    __nanosleep(20);
+                    if (++polls > (1u << 22)) {
+                        raise_error(a.err, B2_ERR_TIMEOUT);
+                        ok = false;
+                    }
+                }
+                // everything issued has completed before tensor memory is freed
+                umma_commit(done);
+                mbar_wait_bounded(done, 0, a.err);
+            }
+            __syncwarp();
+        }
+    } else if (warp >= (uint32_t)kRowsSoftWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRowsConvRegs));
+        // ---- ring tiles into operands ----
+        // Every warp takes part in every tile's K, or in every tile's V, so none can be two
+        // phases of a barrier away from the others. K and V differ in how a lane picks its
+        // values; the conversion of its HD / 32 chunks of eight (16 bytes of hi, 16 of lo) is
+        // one piece of code for both: the roles of this kernel run different code side by
+        // side, and instruction fetch is what they run out of first.
+        constexpr int U = HD / 4;  // values a lane holds of eight places
+        const uint32_t key = lane & 7, c0 = ((lane >> 3) + key) & 3, swap = key & 4;
+        const bool is_v = warp >= (uint32_t)kRowsSoftWarps + 4;
+        for (uint32_t j = 0; j < nt; ++j) {
+            const uint32_t i = 2 * j + is_v, sl = i % NR;
+            const uint32_t st = is_v ? j % VST : j % KST, pass = is_v ? j / VST : j / KST;
+            if (!warp_wait(&r_full[sl], i / NR, a.err)) break;
+            if (pass > 0 && !warp_wait((is_v ? v_empty : k_empty) + st, pass - 1, a.err)) break;
+            const uint64_t hide = rhide[sl];
+#pragma unroll 1
+            for (uint32_t w = (warp & 3) * (kRowsUnit / 8), we = w + kRowsUnit / 8; w < we; ++w) {
+                const uint32_t place = (t0 + j) * kRowsKeys + 8 * w;
+                // places past the end (never copied) and on bad pages are zeros, hidden from every row
+                uint32_t none = (uint32_t)(hide >> (8 * w)) & 0xFFu, bad = 0;
+                if (place + 8 > places) none |= places <= place ? 0xFFu : (0xFFu << (places - place)) & 0xFFu;
+                const float *src = reinterpret_cast<const float *>(smem + S::off_r + sl * S::slot) + 8 * w * hd;
+                float x[U];
+                uint32_t first;  // dimension of the lane's first chunk (V: of its first column)
+                if (!is_v) {
+                    // the lane's key is `key`, its chunks of eight dimensions c0, c0 + 4, ..; the rotation by
+                    // the key and the swapped halves keep the reads of eight rows and the writes of one
+                    // 16-byte column each free of bank conflicts
+                    first = 8 * c0;
+                    const float *from = src + key * hd + 8 * c0;
+#pragma unroll
+                    for (int k = 0; k < HD / 32; ++k) {
+                        const float *at = EXACT || 32 * k + 8 * c0 < hd ? from + 32 * k : from - 8 * c0;
+                        const float4 f = *reinterpret_cast<const float4 *>(at + swap), g = *reinterpret_cast<const float4 *>(at + (swap ^ 4));
+                        x[8 * k] = swap ? g.x : f.x, x[8 * k + 1] = swap ? g.y : f.y, x[8 * k + 2] = swap ? g.z : f.z,
+                        x[8 * k + 3] = swap ? g.w : f.w, x[8 * k + 4] = swap ? f.x : g.x, x[8 * k + 5] = swap ? f.y : g.y,
+                        x[8 * k + 6] = swap ? f.z : g.z, x[8 * k + 7] = swap ? f.w : g.w;
+                    }
+                } else {
+                    // dimensions lane + 32 k of the eight places
+                    first = lane;
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+#pragma unroll
+                        for (int k = 0; k < HD / 32; ++k)
+                            x[8 * k + c] = src[c * hd + (EXACT || lane + 32 * k < hd ? lane + 32 * k : 0)];
+                }
+                if (none != 0) {
+#pragma unroll
+                    for (int k = 0; k < U; ++k)
+                        if (none >> (is_v ? k & 7 : key) & 1) x[k] = 0.0f;
+                }
+                float big = 0.0f;
+#pragma unroll
+                for (int k = 0; k < U; k += 2) big = max3_nan(big, fabsf(x[k]), fabsf(x[k + 1]));
+                uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(big));  // a NaN's bits are above infinity's
+                if (top >= 0x7F800000u) {  // a NaN or infinity: zero it, mark its place
+                    top = 0;
+#pragma unroll
+                    for (int k = 0; k < U; ++k) {
+                        if (abs_bits(x[k]) >= 0x7F800000u) {
+                            bad |= 1u << (is_v ? k & 7 : key);
+                            x[k] = 0.0f;
+                        }
+                        top = max(top, abs_bits(x[k]));
+                    }
+                    top = __reduce_max_sync(0xffffffffu, top);
+                    bad = __reduce_or_sync(0xffffffffu, bad);
+                }
+                const int e = top_exp(top);
+                if (e != kRowsTop) {
+                    const float sc = pow2i(kRowsTop - e);
+                    const uint64_t sc2 = pair(sc, sc);
+#pragma unroll
+                    for (int k = 0; k < U; k += 2) unpair(mul2(pair(x[k], x[k + 1]), sc2), x[k], x[k + 1]);
+                }
+                // element (key, d) of K: chunk d / 8 of 64 rows; (d, place) of V: chunk place / 8 of HD rows
+                uint8_t *dst = smem + (is_v ? S::off_v + st * 2 * S::half + w * (HD * 16) + lane * 16
+                                            : S::off_k + st * 2 * S::half + c0 * (kRowsKeys * 16) + w * 128 + key * 16);
+                const uint32_t step = is_v ? 32 * 16 : 4 * (kRowsKeys * 16);
+#pragma unroll
+                for (uint32_t k = 0; k < HD / 32; ++k) {
+                    if (EXACT || first + 32 * k < hd) {
+                        uint4 h, l;
+                        split_f16(x[8 * k], x[8 * k + 1], h.x, l.x);
+                        split_f16(x[8 * k + 2], x[8 * k + 3], h.y, l.y);
+                        split_f16(x[8 * k + 4], x[8 * k + 5], h.z, l.z);
+                        split_f16(x[8 * k + 6], x[8 * k + 7], h.w, l.w);
+                        *reinterpret_cast<uint4 *>(dst + k * step) = h;
+                        *reinterpret_cast<uint4 *>(dst + k * step + S::half) = l;
+                    }
+                }
+                if (lane == 0) (is_v ? vmeta + st * 8 : kmeta + (j % kRowsMeta) * 8)[w] = unit_meta(e, none, bad);
             }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
-                (is_v ? vmeta + st * 8 : kmeta + (j % kRowsMeta) * 8)[w] = unit_meta(e, none, bad);
+                mbar_arrive(&r_empty[sl]);
                 mbar_arrive((is_v ? v_full : k_full) + st);
             }
         }
-    } else if (warp == kRowsMmaWarp) {
-        // ---- MMA issue ----
-        if (lane == 0) {
-            const uint32_t id_s = umma_idesc_f16(kRowsM, kRowsKeys), id_o = umma_idesc_f16(kRowsM, hd);
-            const uint32_t kb = smem_u32(smem + S::off_k), vb = smem_u32(smem + S::off_v);
-            // S of tile js and O of tile jo, whichever has its operands: K of the next tile
-            // and P of this one are ready in either order
-            bool ok = mbar_wait_bounded(q_full, 0, a.err);
-            uint32_t js = 0, jo = 0, polls = 0;
-            while (ok && jo < nt) {
-                const uint32_t ks = js % KST, vs = jo % VST, ob = jo & 1;
-                if (js < nt && mbar_try_wait(&k_full[ks], (js / KST) & 1) && (js == 0 || mbar_try_wait(s_empty, (js - 1) & 1))) {
-                    tc_fence_after();
-                    const uint32_t kt = kb + ks * 2 * S::half;
-                    // (a descriptor's address field counts 16 bytes)
-                    uint64_t kh = umma_desc(kt, kRowsKeys * 16, 128), kl = umma_desc(kt + S::half, kRowsKeys * 16, 128);
-#pragma unroll 1
-                    for (uint32_t kk = 0; kk < hd / 16; ++kk, kh += 2 * kRowsKeys, kl += 2 * kRowsKeys) {
-                        umma_16_ts(tm_s, tm_q + kk * 8, kh, id_s, kk > 0);
-                        umma_16_ts(tm_s, tm_q + HD / 2 + kk * 8, kh, id_s, 1);
-                        umma_16_ts(tm_s, tm_q + kk * 8, kl, id_s, 1);
-                    }
-                    umma_commit(s_full);
-                    umma_commit(&k_empty[ks]);
-                    ++js;
-                    polls = 0;
-                }
-                if (jo < js && mbar_try_wait(p_full, jo & 1) && mbar_try_wait(&v_full[vs], (jo / VST) & 1) &&
-                    (jo < 2 || mbar_try_wait(&o_empty[ob], (jo / 2 - 1) & 1))) {
-                    tc_fence_after();
-                    const uint32_t d = tm_o + ob * HD, vt = vb + vs * 2 * S::half;
-                    uint64_t vh = umma_desc(vt, HD * 16, 128), vl = umma_desc(vt + S::half, HD * 16, 128);
-#pragma unroll 1
-                    for (uint32_t kk = 0; kk < kRowsKeys / 16; ++kk, vh += 2 * HD, vl += 2 * HD) {
-                        umma_16_ts(d, tm_p + kk * 8, vh, id_o, kk > 0);
-                        umma_16_ts(d, tm_p + 32 + kk * 8, vh, id_o, 1);
-                        umma_16_ts(d, tm_p + kk * 8, vl, id_o, 1);
-                    }
-                    umma_commit(&o_full[ob]);
-                    umma_commit(&v_empty[vs]);
-                    ++jo;
-                    polls = 0;
-                }
-                if (++polls > (1u << 22)) {
-                    raise_error(a.err, B2_ERR_TIMEOUT);
-                    ok = false;
-                }
-            }
-            // everything issued has completed before tensor memory is freed
-            umma_commit(done);
-            mbar_wait_bounded(done, 0, a.err);
-        }
-        __syncwarp();
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowsSoftRegs));
         const uint32_t qt = warp & 3, half = warp >> 2;
         if (qt < nsoft / 2) {
             // ---- softmax and the sums of O: row r, places 32 half .. + 31, dimensions of half ----
@@ -645,7 +674,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 }
                 uint32_t hi[16], lo[16];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) split_f16(s[2 * k], s[2 * k + 1], hi[k], lo[k]);
+                for (int k = 0; k < 16; ++k) cut_f16(s[2 * k], s[2 * k + 1], hi[k], lo[k]);
                 if (j > 0) {
                     wait(&o_full[(j - 1) & 1], (j - 1) / 2);  // P is free, and O of tile j - 1 is there
                     tc_fence_after();
