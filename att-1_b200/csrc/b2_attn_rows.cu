@@ -67,11 +67,12 @@ constexpr uint32_t kRowsUnit = 16;      // places a converting warp takes of a t
 constexpr uint32_t kRowsMeta = 8;       // ring of per-tile scales: more than the tiles between converting and softmax
 constexpr uint32_t kRowsMaxSplits = 64;
 constexpr int kRowsTop = 0;             // operands are scaled to [2^kRowsTop, 2^(kRowsTop + 4))
-constexpr float kRowsP = 12.0f;         // P is scaled by 2^12
+constexpr float kRowsP = 11.0f;         // P is scaled by 2^11,
+constexpr float kRowsSlack = 4.0f;      // and may pass that by 2^4 (f16 ends at 2^16) before the maximum is raised
 
 template <int HD>
 struct RowsSmem {
-    static constexpr uint32_t k_stages = 2, v_stages = 2;
+    static constexpr uint32_t k_stages = 2, v_stages = 2, o_bufs = HD == 128 ? 1 : 2;
     static constexpr uint32_t slots = HD == 128 ? 3 : 6;           // ring of f32 tiles, K and V in turn
     static constexpr uint32_t slot = kRowsKeys * HD * 4;
     static constexpr uint32_t half = kRowsKeys * HD * 2;           // hi or lo of an operand
@@ -134,38 +135,6 @@ __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t
 // floored so that the scale 2^(kRowsTop - e) and its inverse stay normal.
 __device__ __forceinline__ int top_exp(uint32_t amax_bits) { return max(((int)(amax_bits >> 23) - 127) & ~3, -100); }
 
-// f16 hi and lo words of two values.
-__device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32_t &lo)
-{
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
-}
-
-// The same with hi cut off instead of rounded (a mask instead of a conversion
-// back): 21 bits together, for the weights, whose lo is then never negative.
-__device__ __forceinline__ void cut_f16(float a, float b, uint32_t &hi, uint32_t &lo)
-{
-    const float ha = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u), hb = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
-    const __half2 h = __floats2half2_rn(ha, hb), l = __floats2half2_rn(a - ha, b - hb);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
-}
-
-// What the softmax needs to know of a unit: exponent, places hidden from every
-// row, places with a NaN or infinity.
-__device__ __forceinline__ uint32_t unit_meta(int e, uint32_t hidden, uint32_t bad) { return (uint32_t)(e + 128) << 16 | hidden << 8 | bad; }
-__device__ __forceinline__ int meta_exp(uint32_t m) { return (int)(m >> 16) - 128; }
-// byte i of the result: (m_i >> shift) & 0xFF
-__device__ __forceinline__ uint32_t meta_bytes(const uint4 &m, uint32_t shift)
-{
-    return (m.x >> shift & 0xFF) | (m.y >> shift & 0xFF) << 8 | (m.z >> shift & 0xFF) << 16 | (m.w >> shift & 0xFF) << 24;
-}
-// Four units that share an exponent and have nothing marked.
-__device__ __forceinline__ bool meta_plain(const uint4 &m) { return m.x == m.y && m.x == m.z && m.x == m.w && (m.x & 0xFFFF) == 0; }
-
 // Two f32 in one register pair.
 __device__ __forceinline__ uint64_t pair(float a, float b)
 {
@@ -193,6 +162,48 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
     return r;
 }
 
+// f16 hi and lo words of two values.
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32_t &lo)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    float x, y;
+    unpair(fma2(pair(f.x, f.y), pair(-1.0f, -1.0f), pair(a, b)), x, y);  // exact
+    const __half2 l = __floats2half2_rn(x, y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// The same with hi cut off instead of rounded (a mask instead of a conversion
+// back): 21 bits together, for the weights, whose lo is then never negative.
+__device__ __forceinline__ void cut_f16(float a, float b, uint32_t &hi, uint32_t &lo)
+{
+    const float ha = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u), hb = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
+    float x, y;
+    unpair(fma2(pair(ha, hb), pair(-1.0f, -1.0f), pair(a, b)), x, y);  // exact
+    const __half2 h = __floats2half2_rn(ha, hb), l = __floats2half2_rn(x, y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// What the softmax needs to know of a unit: exponent, places hidden from every
+// row, places with a NaN or infinity.
+__device__ __forceinline__ uint32_t unit_meta(int e, uint32_t hidden, uint32_t bad) { return (uint32_t)(e + 128) << 16 | hidden << 8 | bad; }
+__device__ __forceinline__ int meta_exp(uint32_t m) { return (int)(m >> 16) - 128; }
+// byte i of the result: (m_i >> shift) & 0xFF
+__device__ __forceinline__ uint32_t meta_bytes(const uint4 &m, uint32_t shift)
+{
+    return (m.x >> shift & 0xFF) | (m.y >> shift & 0xFF) << 8 | (m.z >> shift & 0xFF) << 16 | (m.w >> shift & 0xFF) << 24;
+}
+// Four units that share an exponent and have nothing marked.
+__device__ __forceinline__ bool meta_plain(const uint4 &m) { return m.x == m.y && m.x == m.z && m.x == m.w && (m.x & 0xFFFF) == 0; }
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 // Largest of three, NaN if one is.
 __device__ __forceinline__ float max3_nan(float a, float b, float c)
 {
@@ -212,6 +223,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
                  : "r"(taddr)
                  : "memory");
 }
+__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16])
 {
     asm volatile(
@@ -223,6 +243,20 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// Whether a phase is over, without the wait of mbar_try_wait.
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // All lanes wait; false for the whole warp if any gave up.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase, int32_t *err)
 {
@@ -233,7 +267,7 @@ template <int HD, bool EXACT>
 __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsParams p)
 {
     using S = RowsSmem<HD>;
-    constexpr uint32_t KST = S::k_stages, VST = S::v_stages, NR = S::slots;
+    constexpr uint32_t KST = S::k_stages, VST = S::v_stages, NR = S::slots, OB = S::o_bufs;
     extern __shared__ __align__(1024) uint8_t smem[];
     const b2_attn_rows_args &a = p.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -294,8 +328,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    // columns: S 64 | P hi 32, lo 32 | Q hi HD / 2, lo HD / 2 | O from 256, two buffers of HD
-    const uint32_t tm_s = tmem, tm_p = tmem + 64, tm_q = tmem + 128, tm_o = tmem + 256;
+    // columns: S with K's hi 64, with its lo 64 | P hi 32, lo 32 | Q hi HD / 2, lo HD / 2 | O from 320
+    const uint32_t tm_s = tmem, tm_p = tmem + 128, tm_q = tmem + 192, tm_o = tmem + 320;
 
     if (warp >= kRowsMmaWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRowsLastRegs));
@@ -355,32 +389,32 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
         } else if (warp == kRowsMmaWarp) {
             // ---- MMA issue ----
             if (lane == 0) {
-                const uint32_t id_s = umma_idesc_f16(kRowsM, kRowsKeys), id_o = umma_idesc_f16(kRowsM, hd);
+                const uint32_t id_s2 = umma_idesc_f16(kRowsM, 2 * kRowsKeys), id_s = umma_idesc_f16(kRowsM, kRowsKeys),
+                           id_o = umma_idesc_f16(kRowsM, hd);
                 const uint32_t kb = smem_u32(smem + S::off_k), vb = smem_u32(smem + S::off_v);
                 // S of tile js and O of tile jo, whichever has its operands: K of the next tile
                 // and P of this one are ready in either order
                 bool ok = mbar_wait_bounded(q_full, 0, a.err);
                 uint32_t js = 0, jo = 0, polls = 0;
                 while (ok && jo < nt) {
-                    const uint32_t ks = js % KST, vs = jo % VST, ob = jo & 1;
-                    if (js < nt && mbar_try_wait(&k_full[ks], (js / KST) & 1) && (js == 0 || mbar_try_wait(s_empty, (js - 1) & 1))) {
+                    const uint32_t ks = js % KST, vs = jo % VST, ob = jo % OB;
+                    if (js < nt && mbar_test(&k_full[ks], (js / KST) & 1) && (js == 0 || mbar_test(s_empty, (js - 1) & 1))) {
                         tc_fence_after();
                         const uint32_t kt = kb + ks * 2 * S::half;
                         // (a descriptor's address field counts 16 bytes)
-                        uint64_t kh = umma_desc(kt, kRowsKeys * 16, 128), kl = umma_desc(kt + S::half, kRowsKeys * 16, 128);
+                        uint64_t kd = umma_desc(kt, 2 * kRowsKeys * 16, 128);  // 64 rows of hi, 64 of lo
 #pragma unroll 1
-                        for (uint32_t kk = 0; kk < hd / 16; ++kk, kh += 2 * kRowsKeys, kl += 2 * kRowsKeys) {
-                            umma_16_ts(tm_s, tm_q + kk * 8, kh, id_s, kk > 0);
-                            umma_16_ts(tm_s, tm_q + HD / 2 + kk * 8, kh, id_s, 1);
-                            umma_16_ts(tm_s, tm_q + kk * 8, kl, id_s, 1);
+                        for (uint32_t kk = 0; kk < hd / 16; ++kk, kd += 4 * kRowsKeys) {
+                            umma_16_ts(tm_s, tm_q + kk * 8, kd, id_s2, kk > 0);
+                            umma_16_ts(tm_s, tm_q + HD / 2 + kk * 8, kd, id_s, 1);  // the hi rows
                         }
                         umma_commit(s_full);
                         umma_commit(&k_empty[ks]);
                         ++js;
                         polls = 0;
                     }
-                    if (jo < js && mbar_try_wait(p_full, jo & 1) && mbar_try_wait(&v_full[vs], (jo / VST) & 1) &&
-                        (jo < 2 || mbar_try_wait(&o_empty[ob], (jo / 2 - 1) & 1))) {
+                    if (jo < js && mbar_test(p_full, jo & 1) && mbar_test(&v_full[vs], (jo / VST) & 1) &&
+                        (jo < OB || mbar_test(&o_empty[ob], (jo / OB - 1) & 1))) {
                         tc_fence_after();
                         const uint32_t d = tm_o + ob * HD, vt = vb + vs * 2 * S::half;
                         uint64_t vh = umma_desc(vt, HD * 16, 128), vl = umma_desc(vt + S::half, HD * 16, 128);
@@ -485,10 +519,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
 #pragma unroll
                     for (int k = 0; k < U; k += 2) unpair(mul2(pair(x[k], x[k + 1]), sc2), x[k], x[k + 1]);
                 }
-                // element (key, d) of K: chunk d / 8 of 64 rows; (d, place) of V: chunk place / 8 of HD rows
+                // element (key, d) of K: chunk d / 8 of 128 rows (64 hi, 64 lo); (d, place) of V: chunk place / 8 of HD rows
                 uint8_t *dst = smem + (is_v ? S::off_v + st * 2 * S::half + w * (HD * 16) + lane * 16
-                                            : S::off_k + st * 2 * S::half + c0 * (kRowsKeys * 16) + w * 128 + key * 16);
-                const uint32_t step = is_v ? 32 * 16 : 4 * (kRowsKeys * 16);
+                                            : S::off_k + st * 2 * S::half + c0 * (2 * kRowsKeys * 16) + w * 128 + key * 16);
+                const uint32_t step = is_v ? 32 * 16 : 4 * (2 * kRowsKeys * 16), to_lo = is_v ? S::half : kRowsKeys * 16;
 #pragma unroll
                 for (uint32_t k = 0; k < HD / 32; ++k) {
                     if (EXACT || first + 32 * k < hd) {
@@ -498,7 +532,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                         split_f16(x[8 * k + 4], x[8 * k + 5], h.z, l.z);
                         split_f16(x[8 * k + 6], x[8 * k + 7], h.w, l.w);
                         *reinterpret_cast<uint4 *>(dst + k * step) = h;
-                        *reinterpret_cast<uint4 *>(dst + k * step + S::half) = l;
+                        *reinterpret_cast<uint4 *>(dst + k * step + to_lo) = l;
                     }
                 }
                 if (lane == 0) (is_v ? vmeta + st * 8 : kmeta + (j % kRowsMeta) * 8)[w] = unit_meta(e, none, bad);
@@ -562,7 +596,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
             auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + qt) : "memory"); };
             // O of tile i into the sums: acc = acc * corr + O * osc
             auto take_o = [&](uint32_t i) {
-                const uint32_t col = tm_o + lanes + (i & 1) * HD + half * (HD / 2);
+                const uint32_t col = tm_o + lanes + (i % OB) * HD + half * (HD / 2);
                 tc_fence_after();
                 if (!__all_sync(0xffffffffu, corr_prev == 1.0f || !mine)) {
                     const uint64_t c2 = pair(corr_prev, corr_prev);
@@ -570,18 +604,16 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                     for (int k = 0; k < HD / 4; ++k) acc[k] = mul2(acc[k], c2);
                 }
                 const uint64_t o2 = pair(osc_prev, osc_prev);
+                uint32_t v[HD / 2];
+                tmem_ld32(col, *reinterpret_cast<uint32_t(*)[32]>(v));
+                if constexpr (HD == 128) tmem_ld32(col + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+                tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < HD / 2; c += 32) {
-                    uint32_t v[32];
-                    tmem_ld32(col + c, v);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int k = 0; k < 16; ++k)
-                        acc[c / 2 + k] = fma2(pair(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), o2, acc[c / 2 + k]);
-                }
+                for (int k = 0; k < HD / 4; ++k)
+                    acc[k] = fma2(pair(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), o2, acc[k]);
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&o_empty[i & 1]);
+                if (lane == 0) mbar_arrive(&o_empty[i % OB]);
             };
             // places of the 32 from key0 that this row sees
             auto visible = [&](uint32_t key0) -> uint32_t {
@@ -607,16 +639,26 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 const uint32_t mt = j % kRowsMeta, vt = j % VST, key0 = (t0 + j) * kRowsKeys + half * 32;
                 wait(s_full, j);
                 tc_fence_after();
-                uint32_t raw[32];
+                uint32_t raw[32], low[16];
                 tmem_ld32(tm_s + lanes + half * 32, raw);
+                tmem_ld16_nowait(tm_s + lanes + kRowsKeys + half * 32, low);
                 const uint4 km = *reinterpret_cast<const uint4 *>(kmeta + mt * 8 + half * 4);
+                float s[32];
+                tmem_wait_ld();
+                auto sum16 = [&](int k0) {
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2)
+                        unpair(add2(pair(__uint_as_float(raw[k0 + k]), __uint_as_float(raw[k0 + k + 1])),
+                                    pair(__uint_as_float(low[k]), __uint_as_float(low[k + 1]))),
+                               s[k0 + k], s[k0 + k + 1]);
+                };
+                sum16(0);
+                tmem_ld16_nowait(tm_s + lanes + kRowsKeys + half * 32 + 16, low);
                 tmem_wait_ld();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_empty);
-                float s[32];
-#pragma unroll
-                for (int k = 0; k < 32; ++k) s[k] = __uint_as_float(raw[k]);
+                sum16(16);
                 int ks = meta_exp(km.x);
                 uint32_t vis = key0 + 32 > ctx ? visible(key0) : 0xFFFFFFFFu;
                 if (!meta_plain(km)) {  // units of different scale, places hidden or not finite
@@ -635,15 +677,21 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                     for (int k = 0; k < 32; ++k)
                         if (!(vis >> k & 1)) s[k] = -INFINITY;
                 }
-                float top = fmaxf(s[0], s[1]);
+                float top = fmaxf(s[0], s[1]), top2 = fmaxf(s[2], s[3]);
 #pragma unroll
-                for (int k = 2; k < 32; k += 2) top = fmaxf(top, fmaxf(s[k], s[k + 1]));
+                for (int k = 4; k < 32; k += 4) {
+                    top = max3(top, s[k], s[k + 1]);
+                    top2 = max3(top2, s[k + 2], s[k + 3]);
+                }
+                top = fmaxf(top, top2);
                 const float cqk = cq * pow2i(ks - kRowsTop);
                 // the row's maximum over both halves
                 float *x = xmax + (j & 1) * 2 * kRowsM;
                 x[half * kRowsM + r] = top * cqk;
                 meet();
-                const float m_new = fmaxf(m, fmaxf(top * cqk, x[(half ^ 1) * kRowsM + r]));
+                // (kept while it grows by less than kRowsSlack, so that the sums are seldom rescaled)
+                float m_new = fmaxf(top * cqk, x[(half ^ 1) * kRowsM + r]);
+                m_new = m_new > m + kRowsSlack ? m_new : m;
                 const float m_use = m_new == -INFINITY ? 0.0f : m_new;
                 const float corr = ex2(m - m_use);
                 m = m_new;
@@ -676,7 +724,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
 #pragma unroll
                 for (int k = 0; k < 16; ++k) cut_f16(s[2 * k], s[2 * k + 1], hi[k], lo[k]);
                 if (j > 0) {
-                    wait(&o_full[(j - 1) & 1], (j - 1) / 2);  // P is free, and O of tile j - 1 is there
+                    wait(&o_full[(j - 1) % OB], (j - 1) / OB);  // P is free, and O of tile j - 1 is there
                     tc_fence_after();
                 }
                 tmem_st16(tm_p + lanes + half * 16, hi);
@@ -689,7 +737,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 corr_prev = corr;
                 osc_prev = pow2i(emax - kRowsTop - (int)kRowsP);
             }
-            wait(&o_full[(nt - 1) & 1], (nt - 1) / 2);
+            wait(&o_full[(nt - 1) % OB], (nt - 1) / OB);
             take_o(nt - 1);
             // the row's sum: both halves', in one order
             float *x = xmax + (nt & 1) * 2 * kRowsM;
