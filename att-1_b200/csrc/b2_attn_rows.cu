@@ -72,19 +72,19 @@ constexpr float kRowsSlack = 4.0f;      // and may pass that by 2^4 (f16 ends at
 
 template <int HD>
 struct RowsSmem {
-    static constexpr uint32_t k_stages = 2, v_stages = 2, o_bufs = HD == 128 ? 1 : 2;
+    static constexpr uint32_t stages = 2;                           // operands of two tiles
     static constexpr uint32_t slots = HD == 128 ? 3 : 6;           // ring of f32 tiles, K and V in turn
     static constexpr uint32_t slot = kRowsKeys * HD * 4;
     static constexpr uint32_t half = kRowsKeys * HD * 2;           // hi or lo of an operand
     static constexpr uint32_t off_k = 0;
-    static constexpr uint32_t off_v = off_k + k_stages * 2 * half;
-    static constexpr uint32_t off_r = off_v + v_stages * 2 * half;
+    static constexpr uint32_t off_v = off_k + stages * 2 * half;
+    static constexpr uint32_t off_r = off_v + stages * 2 * half;
     static constexpr uint32_t off_x = off_r + slots * slot;         // [2][2][128] f32: the halves' maxima, by tile parity
     static constexpr uint32_t off_km = off_x + 4 * kRowsM * 4;      // [kRowsMeta][8] u32: a K unit's exponent and marks
     static constexpr uint32_t off_vm = off_km + kRowsMeta * 8 * 4;  // [2][8] u32: the same of V
     static constexpr uint32_t off_rh = off_vm + 2 * 8 * 4;          // [slots] u64: places whose page is bad
     static constexpr uint32_t off_bar = off_rh + 8 * slots;
-    static constexpr uint32_t bytes = off_bar + 8 * (2 * slots + 2 * k_stages + 2 * v_stages + 9) + 16;
+    static constexpr uint32_t bytes = off_bar + 8 * (2 * slots + 12) + 16;
 };
 static_assert(RowsSmem<128>::bytes <= 227 * 1024 && RowsSmem<64>::bytes <= 227 * 1024, "shared memory");
 
@@ -243,18 +243,22 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// Whether a phase is over, without the wait of mbar_try_wait.
-__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity)
+// mbar_wait_bounded of one thread without the suspension of mbar_try_wait.
+__device__ __forceinline__ bool spin_wait(uint64_t *bar, uint32_t parity, int32_t *err)
 {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
+    for (uint32_t i = 0; i < (1u << 26); ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+    }
+    raise_error(err, B2_ERR_TIMEOUT);
+    return false;
 }
 
 // All lanes wait; false for the whole warp if any gave up.
@@ -267,7 +271,7 @@ template <int HD, bool EXACT>
 __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsParams p)
 {
     using S = RowsSmem<HD>;
-    constexpr uint32_t KST = S::k_stages, VST = S::v_stages, NR = S::slots, OB = S::o_bufs;
+    constexpr uint32_t NR = S::slots;
     extern __shared__ __align__(1024) uint8_t smem[];
     const b2_attn_rows_args &a = p.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -276,10 +280,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
     float *xmax = reinterpret_cast<float *>(smem + S::off_x);
     uint32_t *kmeta = reinterpret_cast<uint32_t *>(smem + S::off_km), *vmeta = reinterpret_cast<uint32_t *>(smem + S::off_vm);
     uint64_t *rhide = reinterpret_cast<uint64_t *>(smem + S::off_rh);
+    // by parity of the tile: K and V converted, S and O computed (which frees that K and V)
     uint64_t *r_full = reinterpret_cast<uint64_t *>(smem + S::off_bar), *r_empty = r_full + NR, *k_full = r_empty + NR,
-             *k_empty = k_full + KST, *v_full = k_empty + KST, *v_empty = v_full + VST, *s_full = v_empty + VST,
-             *s_empty = s_full + 1, *p_full = s_empty + 1, *o_full = p_full + 1, *o_empty = o_full + 2, *q_full = o_empty + 2,
-             *done = q_full + 1;
+             *v_full = k_full + 2, *s_full = v_full + 2, *o_full = s_full + 2, *s_empty = o_full + 2, *p_full = s_empty + 1,
+             *q_full = p_full + 1, *done = q_full + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
 
     pdl_wait();
@@ -304,21 +308,14 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
             mbar_init(&r_full[i], 1);
             mbar_init(&r_empty[i], kRowsKeys / kRowsUnit);
         }
-        for (uint32_t i = 0; i < KST; ++i) {
+        for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(&k_full[i], kRowsKeys / kRowsUnit);
-            mbar_init(&k_empty[i], 1);
-        }
-        for (uint32_t i = 0; i < VST; ++i) {
             mbar_init(&v_full[i], kRowsKeys / kRowsUnit);
-            mbar_init(&v_empty[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&o_full[i], 1);
         }
-        mbar_init(s_full, 1);
         mbar_init(s_empty, nsoft);
         mbar_init(p_full, nsoft);
-        for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(&o_full[i], 1);
-            mbar_init(&o_empty[i], nsoft);
-        }
         mbar_init(q_full, nsoft);
         mbar_init(done, 1);
         fence_mbar_init();
@@ -392,47 +389,37 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 const uint32_t id_s2 = umma_idesc_f16(kRowsM, 2 * kRowsKeys), id_s = umma_idesc_f16(kRowsM, kRowsKeys),
                            id_o = umma_idesc_f16(kRowsM, hd);
                 const uint32_t kb = smem_u32(smem + S::off_k), vb = smem_u32(smem + S::off_v);
-                // S of tile js and O of tile jo, whichever has its operands: K of the next tile
-                // and P of this one are ready in either order
+                // S of tile j + 1 before O of tile j: its operands are there first. (Polling for
+                // whichever came first cost the scheduler's softmax warps more than it gained.)
                 bool ok = mbar_wait_bounded(q_full, 0, a.err);
-                uint32_t js = 0, jo = 0, polls = 0;
-                while (ok && jo < nt) {
-                    const uint32_t ks = js % KST, vs = jo % VST, ob = jo % OB;
-                    if (js < nt && mbar_test(&k_full[ks], (js / KST) & 1) && (js == 0 || mbar_test(s_empty, (js - 1) & 1))) {
+                for (uint32_t j = 0; ok && j <= nt; ++j) {
+                    if (j < nt) {
+                        ok = spin_wait(&k_full[j & 1], (j / 2) & 1, a.err) && (j == 0 || spin_wait(s_empty, (j - 1) & 1, a.err));
+                        if (!ok) break;
                         tc_fence_after();
-                        const uint32_t kt = kb + ks * 2 * S::half;
-                        // (a descriptor's address field counts 16 bytes)
-                        uint64_t kd = umma_desc(kt, 2 * kRowsKeys * 16, 128);  // 64 rows of hi, 64 of lo
+                        // 64 rows of hi, 64 of lo (a descriptor's address field counts 16 bytes)
+                        uint64_t kd = umma_desc(kb + (j & 1) * 2 * S::half, 2 * kRowsKeys * 16, 128);
 #pragma unroll 1
                         for (uint32_t kk = 0; kk < hd / 16; ++kk, kd += 4 * kRowsKeys) {
                             umma_16_ts(tm_s, tm_q + kk * 8, kd, id_s2, kk > 0);
                             umma_16_ts(tm_s, tm_q + HD / 2 + kk * 8, kd, id_s, 1);  // the hi rows
                         }
-                        umma_commit(s_full);
-                        umma_commit(&k_empty[ks]);
-                        ++js;
-                        polls = 0;
+                        umma_commit(&s_full[j & 1]);
                     }
-                    if (jo < js && mbar_test(p_full, jo & 1) && mbar_test(&v_full[vs], (jo / VST) & 1) &&
-                        (jo < OB || mbar_test(&o_empty[ob], (jo / OB - 1) & 1))) {
+                    if (j > 0) {
+                        // P of a tile is published after its V was converted and the O before it taken
+                        const uint32_t i = j - 1, vt = vb + (i & 1) * 2 * S::half;
+                        ok = spin_wait(p_full, i & 1, a.err);
+                        if (!ok) break;
                         tc_fence_after();
-                        const uint32_t d = tm_o + ob * HD, vt = vb + vs * 2 * S::half;
                         uint64_t vh = umma_desc(vt, HD * 16, 128), vl = umma_desc(vt + S::half, HD * 16, 128);
 #pragma unroll 1
                         for (uint32_t kk = 0; kk < kRowsKeys / 16; ++kk, vh += 2 * HD, vl += 2 * HD) {
-                            umma_16_ts(d, tm_p + kk * 8, vh, id_o, kk > 0);
-                            umma_16_ts(d, tm_p + 32 + kk * 8, vh, id_o, 1);
-                            umma_16_ts(d, tm_p + kk * 8, vl, id_o, 1);
+                            umma_16_ts(tm_o, tm_p + kk * 8, vh, id_o, kk > 0);
+                            umma_16_ts(tm_o, tm_p + 32 + kk * 8, vh, id_o, 1);
+                            umma_16_ts(tm_o, tm_p + kk * 8, vl, id_o, 1);
                         }
-                        umma_commit(&o_full[ob]);
-                        umma_commit(&v_empty[vs]);
-                        ++jo;
-                        polls = 0;
-                    }
-                    __nanosleep(20);
-                    if (++polls > (1u << 22)) {
-                        raise_error(a.err, B2_ERR_TIMEOUT);
-                        ok = false;
+                        umma_commit(&o_full[i & 1]);
                     }
                 }
                 // everything issued has completed before tensor memory is freed
@@ -454,9 +441,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
         const bool is_v = warp >= (uint32_t)kRowsSoftWarps + 4;
         for (uint32_t j = 0; j < nt; ++j) {
             const uint32_t i = 2 * j + is_v, sl = i % NR;
-            const uint32_t st = is_v ? j % VST : j % KST, pass = is_v ? j / VST : j / KST;
+            const uint32_t st = j & 1;
             if (!warp_wait(&r_full[sl], i / NR, a.err)) break;
-            if (pass > 0 && !warp_wait((is_v ? v_empty : k_empty) + st, pass - 1, a.err)) break;
+            if (j >= 2 && !warp_wait((is_v ? o_full : s_full) + st, j / 2 - 1, a.err)) break;
             const uint64_t hide = rhide[sl];
 #pragma unroll 1
             for (uint32_t w = (warp & 3) * (kRowsUnit / 8), we = w + kRowsUnit / 8; w < we; ++w) {
@@ -594,26 +581,24 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
             bool ok = true;
             auto wait = [&](uint64_t *bar, uint32_t phase) { ok = ok && warp_wait(bar, phase, a.err); };
             auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + qt) : "memory"); };
-            // O of tile i into the sums: acc = acc * corr + O * osc
-            auto take_o = [&](uint32_t i) {
-                const uint32_t col = tm_o + lanes + (i % OB) * HD + half * (HD / 2);
-                tc_fence_after();
+            // O of the tile before into the sums: acc = acc * corr + O * osc
+            auto take_o = [&]() {
+                const uint32_t col = tm_o + lanes + half * (HD / 2);
                 if (!__all_sync(0xffffffffu, corr_prev == 1.0f || !mine)) {
                     const uint64_t c2 = pair(corr_prev, corr_prev);
 #pragma unroll
                     for (int k = 0; k < HD / 4; ++k) acc[k] = mul2(acc[k], c2);
                 }
                 const uint64_t o2 = pair(osc_prev, osc_prev);
-                uint32_t v[HD / 2];
-                tmem_ld32(col, *reinterpret_cast<uint32_t(*)[32]>(v));
-                if constexpr (HD == 128) tmem_ld32(col + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
-                tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < HD / 4; ++k)
-                    acc[k] = fma2(pair(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), o2, acc[k]);
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&o_empty[i % OB]);
+                for (int c = 0; c < HD / 2; c += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(col + c, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        acc[c / 2 + k] = fma2(pair(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), o2, acc[c / 2 + k]);
+                }
             };
             // places of the 32 from key0 that this row sees
             auto visible = [&](uint32_t key0) -> uint32_t {
@@ -636,8 +621,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 return vis;
             };
             for (uint32_t j = 0; j < nt; ++j) {
-                const uint32_t mt = j % kRowsMeta, vt = j % VST, key0 = (t0 + j) * kRowsKeys + half * 32;
-                wait(s_full, j);
+                const uint32_t mt = j % kRowsMeta, vt = j & 1, key0 = (t0 + j) * kRowsKeys + half * 32;
+                wait(&s_full[j & 1], j / 2);
                 tc_fence_after();
                 uint32_t raw[32], low[16];
                 tmem_ld32(tm_s + lanes + half * 32, raw);
@@ -708,7 +693,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 float sy, sz;
                 unpair(sum, sy, sz);
                 l = fmaf(l, corr, sy + sz);
-                wait(&v_full[vt], j / VST);
+                wait(&v_full[vt], j / 2);
                 const uint4 va = *reinterpret_cast<const uint4 *>(vmeta + vt * 8), vb = *reinterpret_cast<const uint4 *>(vmeta + vt * 8 + 4);
                 int emax = meta_exp(va.x);
                 if (!meta_plain(va) || !meta_plain(vb) || va.x != vb.x) {  // units of different scale, or a NaN or infinity in V
@@ -723,22 +708,21 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) cut_f16(s[2 * k], s[2 * k + 1], hi[k], lo[k]);
-                if (j > 0) {
-                    wait(&o_full[(j - 1) % OB], (j - 1) / OB);  // P is free, and O of tile j - 1 is there
-                    tc_fence_after();
-                }
+                if (j > 0) wait(&o_full[(j - 1) & 1], (j - 1) / 2);  // P is free, and O of the tile before is there
+                tc_fence_after();
                 tmem_st16(tm_p + lanes + half * 16, hi);
                 tmem_st16(tm_p + lanes + 32 + half * 16, lo);
+                if (j > 0) take_o();
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full);
-                if (j > 0) take_o(j - 1);
                 corr_prev = corr;
                 osc_prev = pow2i(emax - kRowsTop - (int)kRowsP);
             }
-            wait(&o_full[(nt - 1) % OB], (nt - 1) / OB);
-            take_o(nt - 1);
+            wait(&o_full[(nt - 1) & 1], (nt - 1) / 2);
+            tc_fence_after();
+            take_o();
             // the row's sum: both halves', in one order
             float *x = xmax + (nt & 1) * 2 * kRowsM;
             x[half * kRowsM + r] = l;
