@@ -9,14 +9,14 @@
 // Work split. The rows of an item times the query heads of one KV head are the
 // rows r = token * group + head of a matrix; CTA (split, KV head and block of
 // 128 such rows, item) takes a contiguous range of the places in tiles of 64, so
-// K and V are read once per 128 rows. Five warpgroups:
+// K and V are read once per 128 rows. 20 warps (two idle), by role:
 //   warp 17       streams K and V (f32) into a ring of tiles with bulk copies, a
 //                 run of places on one page each;
 //   warps 8..15   convert 16 places each of every tile's K (8..11) or V (12..15) from
 //                 the ring into matrix operands;
 //   warp 16       one thread issues the tcgen05 MMAs: S = Q K^T of tile j + 1
-//                 before O = P V of tile j; Q, P, S and O live in tensor memory
-//                 (O in two buffers), only K and V are read from shared memory;
+//                 before O = P V of tile j; Q, P, S and O live in tensor memory,
+//                 only K and V are read from shared memory;
 //   warps 0..7    two per 32 rows: a thread holds one row and 32 of a tile's 64
 //                 places: its scores from tensor memory, the row's running maximum
 //                 (over all 64, so the two need not talk), P back into tensor
@@ -46,10 +46,8 @@
 // from tensor memory, two f16 to a column: 128 rows of A would cost as many
 // shared-memory cycles per MMA as B does, and shared memory is what a tile of 64
 // places uses most (copies in 64 KB, conversion 64 + 64 KB, MMAs 96 KB).
-#include "b2_common.cuh"
+#include "b2_attn_rows.cuh"
 #include "b2_umma.cuh"
-
-#include <cuda_fp16.h>
 
 namespace b2 {
 
@@ -65,10 +63,6 @@ constexpr int kRowsSoftRegs = 136, kRowsConvRegs = 80, kRowsLastRegs = 40;
 static_assert(kRowsThreads == 640 && 256 * kRowsSoftRegs + 256 * kRowsConvRegs + 128 * kRowsLastRegs <= 640 * 96, "register split");
 constexpr uint32_t kRowsUnit = 16;      // places a converting warp takes of a tile
 constexpr uint32_t kRowsMeta = 8;       // ring of per-tile scales: more than the tiles between converting and softmax
-constexpr uint32_t kRowsMaxSplits = 64;
-constexpr int kRowsTop = 0;             // operands are scaled to [2^kRowsTop, 2^(kRowsTop + 4))
-constexpr float kRowsP = 11.0f;         // P is scaled by 2^11,
-constexpr float kRowsSlack = 4.0f;      // and may pass that by 2^4 (f16 ends at 2^16) before the maximum is raised
 
 template <int HD>
 struct RowsSmem {
@@ -87,132 +81,6 @@ struct RowsSmem {
     static constexpr uint32_t bytes = off_bar + 8 * (2 * slots + 12) + 16;
 };
 static_assert(RowsSmem<128>::bytes <= 227 * 1024 && RowsSmem<64>::bytes <= 227 * 1024, "shared memory");
-
-struct RowsParams {
-    b2_attn_rows_args a;
-    uint32_t group, blocks;   // query heads per KV head, 128-row blocks per (item, KV head)
-    uint32_t splits;
-    float scale;              // log2(e) / sqrt(head_dim)
-    float *part;              // splits > 1: [item][KV head][block][split][128][head_dim + 2]
-};
-
-// The rows of an item, or false for lengths that do not fit.
-__device__ __forceinline__ bool rows_item(const b2_attn_rows_args &a, uint32_t item, uint32_t &r0, uint32_t &n, uint32_t &ctx)
-{
-    const int32_t s = a.row_start[item], e = a.row_start[item + 1], c = a.ctx_len[item];
-    if (s < 0 || e < s || (uint32_t)e > a.rows || (uint32_t)(e - s) > a.max_rows || c < 0 || (uint32_t)c > a.max_ctx ||
-        (uint32_t)(e - s) > a.max_ctx - (uint32_t)c || (a.tree != nullptr && e - s > B2_MAX_TREE))
-        return false;
-    r0 = (uint32_t)s;
-    n = (uint32_t)(e - s);
-    ctx = (uint32_t)c;
-    return true;
-}
-
-// Places a block of rows can see, and the tiles [t0, t1) of split s.
-__device__ __forceinline__ uint32_t rows_places(const RowsParams &p, uint32_t n, uint32_t ctx, uint32_t blk)
-{
-    if (p.a.tree != nullptr) return ctx + n;
-    return ctx + min(n, (blk * kRowsM + kRowsM - 1) / p.group + 1);
-}
-__device__ __forceinline__ void rows_range(uint32_t places, uint32_t splits, uint32_t s, uint32_t &t0, uint32_t &t1)
-{
-    const uint32_t nt = (places + kRowsKeys - 1) / kRowsKeys;
-    t0 = (uint32_t)((uint64_t)s * nt / splits);
-    t1 = (uint32_t)((uint64_t)(s + 1) * nt / splits);
-}
-
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126..127
-
-// Exponent of the largest magnitude (its bits), down to a multiple of four and
-// floored so that the scale 2^(kRowsTop - e) and its inverse stay normal.
-__device__ __forceinline__ int top_exp(uint32_t amax_bits) { return max(((int)(amax_bits >> 23) - 127) & ~3, -100); }
-
-// Two f32 in one register pair.
-__device__ __forceinline__ uint64_t pair(float a, float b)
-{
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
-{
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
-{
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
-{
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
-// f16 hi and lo words of two values.
-__device__ __forceinline__ void split_f16(float a, float b, uint32_t &hi, uint32_t &lo)
-{
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    float x, y;
-    unpair(fma2(pair(f.x, f.y), pair(-1.0f, -1.0f), pair(a, b)), x, y);  // exact
-    const __half2 l = __floats2half2_rn(x, y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
-}
-
-// The same with hi cut off instead of rounded (a mask instead of a conversion
-// back): 21 bits together, for the weights, whose lo is then never negative.
-__device__ __forceinline__ void cut_f16(float a, float b, uint32_t &hi, uint32_t &lo)
-{
-    const float ha = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u), hb = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
-    float x, y;
-    unpair(fma2(pair(ha, hb), pair(-1.0f, -1.0f), pair(a, b)), x, y);  // exact
-    const __half2 h = __floats2half2_rn(ha, hb), l = __floats2half2_rn(x, y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
-}
-
-// What the softmax needs to know of a unit: exponent, places hidden from every
-// row, places with a NaN or infinity.
-__device__ __forceinline__ uint32_t unit_meta(int e, uint32_t hidden, uint32_t bad) { return (uint32_t)(e + 128) << 16 | hidden << 8 | bad; }
-__device__ __forceinline__ int meta_exp(uint32_t m) { return (int)(m >> 16) - 128; }
-// byte i of the result: (m_i >> shift) & 0xFF
-__device__ __forceinline__ uint32_t meta_bytes(const uint4 &m, uint32_t shift)
-{
-    return (m.x >> shift & 0xFF) | (m.y >> shift & 0xFF) << 8 | (m.z >> shift & 0xFF) << 16 | (m.w >> shift & 0xFF) << 24;
-}
-// Four units that share an exponent and have nothing marked.
-__device__ __forceinline__ bool meta_plain(const uint4 &m) { return m.x == m.y && m.x == m.z && m.x == m.w && (m.x & 0xFFFF) == 0; }
-
-__device__ __forceinline__ float max3(float a, float b, float c)
-{
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-// Largest of three, NaN if one is.
-__device__ __forceinline__ float max3_nan(float a, float b, float c)
-{
-    float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
 // 32 lanes x 32 columns: thread i gets lane (base + i), columns col..col+31. The
 // registers hold after tmem_wait_ld.
@@ -261,12 +129,6 @@ __device__ __forceinline__ bool spin_wait(uint64_t *bar, uint32_t parity, int32_
     return false;
 }
 
-// All lanes wait; false for the whole warp if any gave up.
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase, int32_t *err)
-{
-    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, phase & 1u, err));
-}
-
 template <int HD, bool EXACT>
 __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsParams p)
 {
@@ -298,7 +160,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
     const uint32_t live = min(kRowsM, mrows - blk * kRowsM);
     const uint32_t places = rows_places(p, n, ctx, blk);
     uint32_t t0, t1;
-    rows_range(places, p.splits, split, t0, t1);
+    rows_range(p, places, split, t0, t1);
     if (t0 == t1) return;  // the joining kernel skips the same splits
     const uint32_t nt = t1 - t0;
     const uint32_t nsoft = 2 * ((live + 31) / 32);  // softmax warps with rows: two per quarter of the rows
@@ -735,11 +597,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 return f;
             };
             if (ok && mine) {
-                // the weights carry 2^12, the sums of O do not
+                // the weights carry 2^11, the sums of O do not
                 const float lw = l * pow2i(-(int)kRowsP);
                 if (p.splits > 1) {
-                    float *dst = p.part + ((((size_t)item * a.n_kv_heads + kvh) * p.blocks + blk) * p.splits + split) * kRowsM * (hd + 4) +
-                                 (size_t)r * (hd + 4);
+                    float *dst = rows_part(p, item, kvh, blk, split) + (size_t)r * (hd + 4);
                     if (half == 0) *reinterpret_cast<float2 *>(dst) = make_float2(m, lw);
                     dst += 4;
 #pragma unroll
@@ -781,26 +642,20 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_rows_join_kernel(const R
     uint32_t r0, n, ctx;
     if (!rows_item(a, item, r0, n, ctx)) return;
     if (m_row >= n * p.group) return;
-    const uint32_t blk = m_row / kRowsM, r = m_row % kRowsM;
+    const uint32_t blk = m_row / p.block, r = m_row % p.block;
     const uint32_t places = rows_places(p, n, ctx, blk);
-    const size_t stride = (size_t)kRowsM * (hd + 4);
-    const float *base = p.part + (((size_t)item * a.n_kv_heads + kvh) * p.blocks + blk) * p.splits * stride + (size_t)r * (hd + 4);
+    const size_t stride = (size_t)p.block * (hd + 4);
+    const float *base = rows_part(p, item, kvh, blk, 0) + (size_t)r * (hd + 4);
+    // (with fewer units than splits the first ones have one each)
+    const uint32_t splits = min(p.splits, (places + p.unit - 1) / p.unit);
     // the splits' statistics, one per lane and pass
     float ms[kRowsMaxSplits / 32], ls[kRowsMaxSplits / 32], top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < (int)kRowsMaxSplits / 32; ++i) {
         const uint32_t s = lane + 32 * i;
-        ms[i] = -INFINITY;
-        ls[i] = 0.0f;
-        if (s < p.splits) {
-            uint32_t t0, t1;
-            rows_range(places, p.splits, s, t0, t1);
-            if (t0 < t1) {
-                const float2 x = *reinterpret_cast<const float2 *>(base + s * stride);
-                ms[i] = x.x;
-                ls[i] = x.y;
-            }
-        }
+        const float2 x = s < splits ? *reinterpret_cast<const float2 *>(base + s * stride) : make_float2(-INFINITY, 0.0f);
+        ms[i] = x.x;
+        ls[i] = x.y;
         top = fmaxf(top, ms[i]);
     }
     top = warp_max(top);
@@ -810,14 +665,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_rows_join_kernel(const R
 #pragma unroll
     for (int i = 0; i < (int)kRowsMaxSplits / 32; ++i) {
         const float f = ex2(ms[i] - top);
-        for (uint32_t s = 32 * i; s < min(p.splits, 32u * (i + 1)); ++s) {
-            const float fs = __shfl_sync(0xffffffffu, f, s - 32 * i), lsum = __shfl_sync(0xffffffffu, ls[i], s - 32 * i);
-            uint32_t t0, t1;
-            rows_range(places, p.splits, s, t0, t1);
-            if (t0 == t1) continue;
+        const uint32_t n32 = splits > 32u * i ? min(splits - 32 * i, 32u) : 0;
+#pragma unroll 4
+        for (uint32_t s = 0; s < n32; ++s) {
+            const float fs = __shfl_sync(0xffffffffu, f, s), lsum = __shfl_sync(0xffffffffu, ls[i], s);
             l = fmaf(lsum, fs, l);
             if (4 * lane < hd) {
-                const float4 x = reinterpret_cast<const float4 *>(base + s * stride + 4)[lane];
+                const float4 x = reinterpret_cast<const float4 *>(base + (32 * i + s) * stride + 4)[lane];
                 o = make_float4(fmaf(x.x, fs, o.x), fmaf(x.y, fs, o.y), fmaf(x.z, fs, o.z), fmaf(x.w, fs, o.w));
             }
         }
@@ -846,37 +700,55 @@ static int attn_rows_check(const b2_attn_rows_args *a)
     if (!kv.k_pool || !kv.v_pool || !kv.page_table || kv.page_tokens == 0 || kv.head_dim != a->head_dim ||
         kv.n_kv_heads != a->n_kv_heads || ((uintptr_t)kv.k_pool & 15) || ((uintptr_t)kv.v_pool & 15))
         return -1;
+    if ((uint64_t)a->max_rows * (a->n_heads / a->n_kv_heads) > 0x7FFFFFFFull) return -1;
     if ((uint64_t)kv.page_tokens * kv.pages_per_seq > 0x7FFFFFFFull || a->max_ctx > kv.page_tokens * kv.pages_per_seq)
         return -1;
     return 0;
 }
 
-// Blocks and splits. A CTA costs about kSetup tiles of time besides its own
-// (launch, q, the pipeline's ends), a split launch about kJoin more for the
-// joining kernel: the split count with the least waves x (tiles + kSetup).
-static void attn_rows_plan(const b2_attn_rows_args *a, uint32_t &blocks, uint32_t &splits)
+// Kernel, blocks and splits. Up to kFewRows rows of an (item, KV head) go to
+// attn_few_kernel, which converts K and V in registers and multiplies with mma.sync: no
+// tensor-memory set-up, no roles to synchronise, no 128-row products for a handful of
+// rows (8B shape: 8 tokens at context 1000 15.3 us against 17.8, one token at context
+// 4096 22.7 against 26.0, 32 sequences of it 217 against 231; with 48 rows of head size
+// 64 it loses, 50 against 29).
+//
+// The splits take the least modelled time, in quarters of a tile's: a CTA costs kSetup
+// besides its tiles (launch, q, the pipeline's ends), joining kJoin and one per split,
+// within a cluster half of kJoin. Measured (8B shape, attn_rows_kernel): context 1000
+// with 8 tokens 8 splits 17.8 us, 16 splits 21.2, 4 19.0; one KV head of the 70B shape,
+// 8 sequences of 30000 18 splits 82.8 us, 12 97.9, 24 98.2.
+static void attn_rows_plan(const b2_attn_rows_args *a, RowsParams &p, bool &few)
 {
-    const uint64_t group = a->n_heads / a->n_kv_heads;
-    blocks = (uint32_t)((a->max_rows * group + kRowsM - 1) / kRowsM);
-    const uint64_t ctas = (uint64_t)a->batch * a->n_kv_heads * blocks, sms = (uint64_t)sm_count();
-    const uint64_t tiles = (a->max_ctx + kRowsKeys - 1) / kRowsKeys;
-    constexpr uint64_t kSetup = 4, kJoin = 3;
+    p.group = a->n_heads / a->n_kv_heads;
+    const uint64_t rows = (uint64_t)a->max_rows * p.group, sms = (uint64_t)sm_count();
+    few = rows <= kFewRows;
+    p.block = !few ? kRowsM : rows <= 16 ? 16 : 32;
+    p.unit = few ? kFewUnit : kRowsKeys;
+    p.blocks = (uint32_t)((rows + p.block - 1) / p.block);
+    const uint64_t ctas = (uint64_t)a->batch * a->n_kv_heads * p.blocks;
+    // a tile: 64 places of a tcgen05 CTA, or a pass of 16 places per warp
+    const uint64_t tile = few ? kFewUnit * kFewWarps : kRowsKeys, tiles = (a->max_ctx + tile - 1) / tile;
+    constexpr uint64_t kSetup = 4 * 4, kJoin = 2 * 4;  // quarters of a tile
     uint64_t best = ~0ull;
-    splits = 1;
-    for (uint64_t s = 1; s <= kRowsMaxSplits && s <= tiles; ++s) {
+    p.splits = 1;
+    for (uint64_t s = 1; s <= kRowsMaxSplits && s <= tiles; s = few ? 2 * s : s + 1) {
         const uint64_t waves = (ctas * s + sms - 1) / sms;
-        const uint64_t cost = waves * ((tiles + s - 1) / s + kSetup) + (s > 1 ? kJoin : 0);
+        // (the few kernel joins up to kFewCluster splits itself)
+        const uint64_t join = s == 1 ? 0 : few && s <= kFewCluster ? kJoin / 2 : kJoin + s;
+        const uint64_t cost = waves * (4 * ((tiles + s - 1) / s) + kSetup) + join;
         if (cost < best) {
             best = cost;
-            splits = (uint32_t)s;
+            p.splits = (uint32_t)s;
         }
     }
+    p.cluster = few && p.splits > 1 && p.splits <= kFewCluster;
 }
 
-static size_t attn_rows_scratch(const b2_attn_rows_args *a, uint32_t blocks, uint32_t splits)
+static size_t attn_rows_scratch(const b2_attn_rows_args *a, const RowsParams &p)
 {
-    if (splits == 1) return 0;
-    return (size_t)a->batch * a->n_kv_heads * blocks * splits * kRowsM * (a->head_dim + 4) * sizeof(float);
+    if (p.splits == 1 || p.cluster) return 0;
+    return (size_t)a->batch * a->n_kv_heads * p.blocks * p.splits * p.block * (a->head_dim + 4) * sizeof(float);
 }
 
 static cudaError_t launch_rows_attn(const void *fn, dim3 grid, int threads, size_t smem, int pdl, cudaStream_t st, const RowsParams &p)
@@ -902,9 +774,10 @@ using namespace b2;
 extern "C" size_t b2_attn_rows_scratch_bytes(const b2_attn_rows_args *a)
 {
     if (attn_rows_check(a) != 0) return 0;
-    uint32_t blocks, splits;
-    attn_rows_plan(a, blocks, splits);
-    return attn_rows_scratch(a, blocks, splits);
+    RowsParams p = {};
+    bool few;
+    attn_rows_plan(a, p, few);
+    return attn_rows_scratch(a, p);
 }
 
 extern "C" int b2_attn_rows(const b2_attn_rows_args *a, void *stream)
@@ -913,24 +786,28 @@ extern "C" int b2_attn_rows(const b2_attn_rows_args *a, void *stream)
     if (rc != 0) return rc;
     RowsParams p = {};
     p.a = *a;
-    p.group = a->n_heads / a->n_kv_heads;
-    attn_rows_plan(a, p.blocks, p.splits);
+    bool few;
+    attn_rows_plan(a, p, few);
     if ((uint64_t)a->n_kv_heads * p.blocks > 65535u) return -9;
-    const size_t need = attn_rows_scratch(a, p.blocks, p.splits);
+    const size_t need = attn_rows_scratch(a, p);
     if (need > 0 && (a->scratch == nullptr || a->scratch_bytes < need || ((uintptr_t)a->scratch & 15))) return -1;
     p.part = (float *)a->scratch;
     p.scale = (float)(1.4426950408889634 / sqrt((double)a->head_dim));
     const cudaStream_t st = (cudaStream_t)stream;
-    const bool wide = a->head_dim > 64;
-    const void *fn = a->head_dim == 128  ? (const void *)attn_rows_kernel<128, true>
-                     : wide              ? (const void *)attn_rows_kernel<128, false>
-                     : a->head_dim == 64 ? (const void *)attn_rows_kernel<64, true>
-                                         : (const void *)attn_rows_kernel<64, false>;
-    const size_t smem = wide ? RowsSmem<128>::bytes : RowsSmem<64>::bytes;
-    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return -8;
-    if (launch_rows_attn(fn, dim3(p.splits, a->n_kv_heads * p.blocks, a->batch), kRowsThreads, smem, a->pdl, st, p) != cudaSuccess)
-        return -8;
-    if (p.splits > 1) {
+    if (few) {
+        if (attn_few_launch(p, st) != cudaSuccess) return -8;
+    } else {
+        const bool wide = a->head_dim > 64;
+        const void *fn = a->head_dim == 128  ? (const void *)attn_rows_kernel<128, true>
+                         : wide              ? (const void *)attn_rows_kernel<128, false>
+                         : a->head_dim == 64 ? (const void *)attn_rows_kernel<64, true>
+                                             : (const void *)attn_rows_kernel<64, false>;
+        const size_t smem = wide ? RowsSmem<128>::bytes : RowsSmem<64>::bytes;
+        if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return -8;
+        if (launch_rows_attn(fn, dim3(p.splits, a->n_kv_heads * p.blocks, a->batch), kRowsThreads, smem, a->pdl, st, p) != cudaSuccess)
+            return -8;
+    }
+    if (p.splits > 1 && !p.cluster) {
         const uint32_t rows = a->max_rows * p.group;
         if (launch_rows_attn((const void *)attn_rows_join_kernel, dim3((rows + kJoinWarps - 1) / kJoinWarps, a->n_kv_heads, a->batch),
                              kJoinWarps * 32, 0, a->pdl, st, p) != cudaSuccess)
