@@ -167,18 +167,22 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const b2_kv_plan_
 
 // ---- b2_rows_append -------------------------------------------------------------------
 
-constexpr int kAppendThreads = 256;
+constexpr uint32_t kAppendThreads = 128;  // twice as many for head sizes above 512
+constexpr uint32_t kAppendBatch = 4;      // heads a thread loads before it stores them
 
 // grid (head parts, rows): a thread owns four dimensions (two RoPE pairs) of a
 // row and takes every hgroups-th head of its part, so the sine and cosine of a
 // pair are computed once per thread, not once per head; q | k | v heads in one
-// sequence of h + 2 hkv. One float4 in, one out per head: bound by HBM for many
-// rows, by one load round trip for few.
-__global__ void __launch_bounds__(kAppendThreads) rows_append_kernel(const b2_rows_append_args a, uint32_t heads_per_part)
+// sequence of h + 2 hkv. One float4 in, one out per head. Bound by one load
+// round trip for few rows and by HBM for many, which takes enough bytes on
+// their way: four heads' loads go out before the row's slot and angles are
+// known (2048 rows of the 8B shape: 19.2 us, 5.2 TB/s; one load at a time 25.4;
+// six 19.0, with 256 threads 20.8, 512 23.3, whose CTAs leave in coarser steps).
+__global__ void __launch_bounds__(2 * kAppendThreads) rows_append_kernel(const b2_rows_append_args a, uint32_t heads_per_part)
 {
     pdl_wait();
     pdl_launch_dependents();
-    const uint32_t hd = a.kv.head_dim, cols = hd / 4, hgroups = kAppendThreads / cols;
+    const uint32_t hd = a.kv.head_dim, cols = hd / 4, hgroups = blockDim.x / cols;
     const uint32_t col = threadIdx.x % cols, hg = threadIdx.x / cols;
     const uint32_t qh = a.q_rows / hd, hkv = a.kv.n_kv_heads, heads = qh + 2 * hkv;
     const uint32_t h0 = blockIdx.x * heads_per_part, h1 = min(heads, h0 + heads_per_part);
@@ -186,7 +190,14 @@ __global__ void __launch_bounds__(kAppendThreads) rows_append_kernel(const b2_ro
     const uint32_t slots = a.pool_pages * a.kv.page_tokens;
     if (hg >= hgroups) return;
     for (uint32_t n = blockIdx.y; n < m; n += gridDim.y) {
-        const float *y = a.y + (size_t)n * a.y_stride;
+        const float *y = a.y + (size_t)n * a.y_stride + 4 * col;
+        float4 x[kAppendBatch];  // asked for before the row's slot, position and angles are known
+        auto load = [&](uint32_t h) {
+#pragma unroll
+            for (uint32_t k = 0; k < kAppendBatch; ++k)
+                if (h + k * hgroups < h1) x[k] = __ldcs(reinterpret_cast<const float4 *>(y + (size_t)(h + k * hgroups) * hd));
+        };
+        load(h0 + hg);
         const int32_t slot = a.slots[n];
         const int32_t pos = a.rope_freq != nullptr ? a.positions[n] : 0;
         if (pos < 0 || (slot >= 0 && (uint32_t)slot >= slots)) {
@@ -201,20 +212,26 @@ __global__ void __launch_bounds__(kAppendThreads) rows_append_kernel(const b2_ro
             sincosf(__fmul_rn((float)pos, a.rope_freq[2 * col]), &s0, &c0);
             sincosf(__fmul_rn((float)pos, a.rope_freq[2 * col + 1]), &s1, &c1);
         }
-        for (uint32_t h = h0 + hg; h < h1; h += hgroups) {
-            float4 x = __ldcs(reinterpret_cast<const float4 *>(y + (size_t)h * hd) + col);
-            if (h < qh + hkv && a.rope_freq != nullptr) {
-                x = make_float4(__fsub_rn(__fmul_rn(x.x, c0), __fmul_rn(x.y, s0)),
-                                __fadd_rn(__fmul_rn(x.x, s0), __fmul_rn(x.y, c0)),
-                                __fsub_rn(__fmul_rn(x.z, c1), __fmul_rn(x.w, s1)),
-                                __fadd_rn(__fmul_rn(x.z, s1), __fmul_rn(x.w, c1)));
-            }
-            if (h < qh) {
-                reinterpret_cast<float4 *>(a.q + (size_t)n * a.q_stride + (size_t)h * hd)[col] = x;
-            } else if (store) {
-                const uint32_t kh = h < qh + hkv ? h - qh : h - qh - hkv;
-                float *pool = h < qh + hkv ? a.kv.k_pool : a.kv.v_pool;
-                reinterpret_cast<float4 *>(pool + ((page * hkv + kh) * a.kv.page_tokens + off) * hd)[col] = x;
+        for (uint32_t hb = h0 + hg; hb < h1; hb += kAppendBatch * hgroups) {
+            if (hb != h0 + hg) load(hb);
+#pragma unroll
+            for (uint32_t k = 0; k < kAppendBatch; ++k) {
+                const uint32_t h = hb + k * hgroups;
+                if (h >= h1) break;
+                float4 v = x[k];
+                if (h < qh + hkv && a.rope_freq != nullptr) {
+                    v = make_float4(__fsub_rn(__fmul_rn(v.x, c0), __fmul_rn(v.y, s0)),
+                                    __fadd_rn(__fmul_rn(v.x, s0), __fmul_rn(v.y, c0)),
+                                    __fsub_rn(__fmul_rn(v.z, c1), __fmul_rn(v.w, s1)),
+                                    __fadd_rn(__fmul_rn(v.z, s1), __fmul_rn(v.w, c1)));
+                }
+                if (h < qh) {
+                    reinterpret_cast<float4 *>(a.q + (size_t)n * a.q_stride + (size_t)h * hd)[col] = v;
+                } else if (store) {
+                    const uint32_t kh = h < qh + hkv ? h - qh : h - qh - hkv;
+                    float *pool = h < qh + hkv ? a.kv.k_pool : a.kv.v_pool;
+                    reinterpret_cast<float4 *>(pool + ((page * hkv + kh) * a.kv.page_tokens + off) * hd)[col] = v;
+                }
             }
         }
     }
@@ -438,7 +455,8 @@ extern "C" int b2_rows_append(const b2_rows_append_args *a, void *stream)
         return -1;
     if ((uint64_t)a->pool_pages * kv.page_tokens > 0x7FFFFFFFull) return -1;
     const uint32_t heads = a->q_rows / kv.head_dim + 2 * kv.n_kv_heads;
-    const uint32_t hgroups = kAppendThreads / (kv.head_dim / 4);
+    const uint32_t threads = kv.head_dim / 4 > kAppendThreads ? 2 * kAppendThreads : kAppendThreads;
+    const uint32_t hgroups = threads / (kv.head_dim / 4);
     // few rows: a row's heads over several CTAs, at least one pass of the head groups each
     uint32_t parts = ((uint32_t)sm_count() + a->m - 1) / a->m;
     const uint32_t most = (heads + hgroups - 1) / hgroups;
@@ -449,7 +467,7 @@ extern "C" int b2_rows_append(const b2_rows_append_args *a, void *stream)
     b2_rows_append_args p = *a;
     void *args[] = {&p, &per};
     return launch_tree((const void *)rows_append_kernel, dim3(parts, a->m < 65535u ? a->m : 65535u),
-                       dim3(kAppendThreads), 0, a->pdl, (cudaStream_t)stream, args) == cudaSuccess
+                       dim3(threads), 0, a->pdl, (cudaStream_t)stream, args) == cudaSuccess
                ? 0
                : -8;
 }

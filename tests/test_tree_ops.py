@@ -559,6 +559,13 @@ def test_append_shapes(b2, torch, h, hkv, hd, page, m):
     assert append_run(b2, torch, h, hkv, hd, page, m, seed=m, pad=4 * (m % 2))[0] == 0
 
 
+@pytest.mark.parametrize("h,hkv,hd", [(2, 1, 1024), (3, 3, 516), (5, 1, 512), (150, 75, 16), (1, 1, 4)])
+@pytest.mark.parametrize("m", [1, 40])
+def test_append_head_sizes(b2, torch, h, hkv, hd, m):
+    """Heads wider than a block's threads take, and more heads than a thread loads at a time."""
+    assert append_run(b2, torch, h, hkv, hd, 16, m, seed=m)[0] == 0
+
+
 def test_append_rows_in_use(b2, torch):
     for live in (0, 1, 5, 9, 40, -3):
         assert append_run(b2, torch, 4, 2, 64, 16, 9, live=live)[0] == 0
