@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
         top = __reduce_max_sync(0xffffffffu, top);
         const bool bad = top >= 0x7F800000u;
         const int e = bad ? 0 : top_exp(top);
-        const float sc = bad ? 0.0f : pow2i(kRowsTop - e);
+        const float sc = bad ? 0.0f : pow2i(-e);
         if (bad) f = make_float4(0, 0, 0, 0);
         if (4 * lane < HD) {
             uint32_t h0, h1, l0, l1;
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
             dst[32 * 4] = l0, dst[32 * 4 + 2] = l1;
         }
         if (lane == 0) {
-            cqs[r] = bad ? NAN : pow2i(e - kRowsTop) * p.scale;
+            cqs[r] = bad ? NAN : pow2i(e) * p.scale;
             masks[r] = mine && a.tree != nullptr ? a.tree[r0 + tok] : 0;
         }
     }
@@ -235,53 +235,40 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
         landed();
         const uint32_t hide = hides[c & 3], none = hide | none0;
         uint32_t kbad = 0;
-        int ke;
+        int ke, kpe = 0;  // exponent of K; if kwide, of place `lane`
+        bool kwide = false;
         {
             float4 x[2][KS];  // the lane's K: place 8 nt + g8, dimensions 16 ks + 4 t4 ..
-            const float *src = reinterpret_cast<const float *>(ring + sl * S::slot) + 4 * t4;
+            float *rows0 = reinterpret_cast<float *>(ring + sl * S::slot);
+            auto load = [&]() -> uint32_t {  // bits of the largest magnitude
+                const float *src = rows0 + 4 * t4;
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
+                for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-                    x[nt][ks] = 16 * ks < (int)hd ? *reinterpret_cast<const float4 *>(src + (8 * nt + g8) * hd + 16 * ks) : make_float4(0, 0, 0, 0);
-            float big = 0.0f;
+                    for (int ks = 0; ks < KS; ++ks)
+                        x[nt][ks] = 16 * ks < (int)hd ? *reinterpret_cast<const float4 *>(src + (8 * nt + g8) * hd + 16 * ks) : make_float4(0, 0, 0, 0);
+                float big = 0.0f;
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
+                for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-                    big = max3_nan(max3_nan(big, fabsf(x[nt][ks].x), fabsf(x[nt][ks].y)), fabsf(x[nt][ks].z), fabsf(x[nt][ks].w));
-            uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(big));
-            if (top >= 0x7F800000u) {  // a NaN or infinity: zero it, mark its place
-                top = 0;
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    bool b = false;
-#pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        float *f = reinterpret_cast<float *>(&x[nt][ks]);
-#pragma unroll
-                        for (int v = 0; v < 4; ++v) {
-                            if (abs_bits(f[v]) >= 0x7F800000u) {
-                                b = true;
-                                f[v] = 0.0f;
-                            }
-                            top = max(top, abs_bits(f[v]));
-                        }
-                    }
-                    if (b) kbad |= 1u << (8 * nt + g8);
-                }
-                kbad = __reduce_or_sync(0xffffffffu, kbad);
-                top = __reduce_max_sync(0xffffffffu, top);
+                    for (int ks = 0; ks < KS; ++ks)
+                        big = max3_nan(max3_nan(big, fabsf(x[nt][ks].x), fabsf(x[nt][ks].y)), fabsf(x[nt][ks].z), fabsf(x[nt][ks].w));
+                return __reduce_max_sync(0xffffffffu, abs_bits(big));
+            };
+            uint32_t top = load();
+            if (__builtin_expect(top >= kRowsWide, 0)) {
+                kwide = settle_places(rows0, kFewUnit, hd, 0, kpe, kbad);
+                top = load();
             }
             ke = top_exp(top);
-            const float sc = pow2i(kRowsTop - ke);
+            const float sc = pow2i(-ke);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 uint32_t h[2][2], lo[2][2];
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt) {
                     float4 f = x[nt][ks];
-                    if (ke != kRowsTop) f = make_float4(f.x * sc, f.y * sc, f.z * sc, f.w * sc);
+                    if (ke != 0) f = make_float4(f.x * sc, f.y * sc, f.z * sc, f.w * sc);
                     split_f16(f.x, f.y, h[nt][0], lo[nt][0]);
                     split_f16(f.z, f.w, h[nt][1], lo[nt][1]);
                 }
@@ -302,13 +289,23 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
         fill();  // into the slot just read
         // ---- softmax: a lane holds columns 8 nt + 2 t4, + 1 of its rows ----
         const bool masked = p0 + kFewUnit > ctx || none != 0 || kbad != 0;
-        const float kf = pow2i(ke - kRowsTop);
+        const float kf = pow2i(ke);
+        if (__builtin_expect(kwide, 0)) {
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    const float f = pow2i(__shfl_sync(0xffffffffu, kpe, 8 * nt + 2 * t4 + v));
+#pragma unroll
+                    for (int i = 0; i < 2 * MT; ++i) s[i / 2][nt][(i & 1) * 2 + v] = s[i / 2][nt][(i & 1) * 2 + v] * cq[i] * f;
+                }
+        }
         float corr[2 * MT];
         bool rescale = false;
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i) {
             float *s0 = &s[i / 2][0][(i & 1) * 2], *s1 = &s[i / 2][1][(i & 1) * 2];
-            const float cqk = cq[i] * kf;
+            const float cqk = kwide ? 1.0f : cq[i] * kf;
             if (masked) {
                 const uint32_t vis = visible((i / 2) * 16 + g8 + (i & 1) * 8, p0) & ~none;
 #pragma unroll
@@ -341,81 +338,98 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
                     for (int v = 0; v < 4; ++v) acc[mt][k][v] *= corr[2 * mt + v / 2];
         }
         uint4 ph[MT], pl[MT];  // P's fragments: rows g8, g8 + 8 of columns 2 t4, then of 8 + 2 t4
+        auto split_p = [&]() {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            cut_f16(s[mt][0][0], s[mt][0][1], ph[mt].x, pl[mt].x);
-            cut_f16(s[mt][0][2], s[mt][0][3], ph[mt].y, pl[mt].y);
-            cut_f16(s[mt][1][0], s[mt][1][1], ph[mt].z, pl[mt].z);
-            cut_f16(s[mt][1][2], s[mt][1][3], ph[mt].w, pl[mt].w);
-        }
+            for (int mt = 0; mt < MT; ++mt) {
+                cut_f16(s[mt][0][0], s[mt][0][1], ph[mt].x, pl[mt].x);
+                cut_f16(s[mt][0][2], s[mt][0][3], ph[mt].y, pl[mt].y);
+                cut_f16(s[mt][1][0], s[mt][1][1], ph[mt].z, pl[mt].z);
+                cut_f16(s[mt][1][2], s[mt][1][3], ph[mt].w, pl[mt].w);
+            }
+        };
+        split_p();
         // ---- O: the lane's V: places 2 t4, 2 t4 + 1, 8 + 2 t4, 9 + 2 t4, dimensions 32 q + 4 g8 .. ----
         sl = (2 * c + 1) % NS;
         landed();
         {
             float4 x[4][QG];
-            const float *src = reinterpret_cast<const float *>(ring + sl * S::slot) + 4 * g8;
+            float *rows0 = reinterpret_cast<float *>(ring + sl * S::slot);
+            uint32_t vbad = 0;
+            int vpe = 0;
+            bool vwide = false;
+            auto load = [&]() -> uint32_t {  // bits of the largest magnitude
+                const float *src = rows0 + 4 * g8;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+                for (int k = 0; k < 4; ++k)
 #pragma unroll
-                for (int q = 0; q < QG; ++q)
-                    x[k][q] = 32 * q + 4 * g8 < hd ? *reinterpret_cast<const float4 *>(src + (2 * t4 + (k & 1) + (k >> 1) * 8) * hd + 32 * q)
-                                                   : make_float4(0, 0, 0, 0);
-            float big = 0.0f;
+                    for (int q = 0; q < QG; ++q)
+                        x[k][q] = 32 * q + 4 * g8 < hd ? *reinterpret_cast<const float4 *>(src + (2 * t4 + (k & 1) + (k >> 1) * 8) * hd + 32 * q)
+                                                       : make_float4(0, 0, 0, 0);
+                float big = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+                for (int k = 0; k < 4; ++k)
 #pragma unroll
-                for (int q = 0; q < QG; ++q)
-                    big = max3_nan(max3_nan(big, fabsf(x[k][q].x), fabsf(x[k][q].y)), fabsf(x[k][q].z), fabsf(x[k][q].w));
-            uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(big));
-            if (top >= 0x7F800000u) {  // zero it; the rows that see its place become NaN
-                uint32_t vbad = 0;
-                top = 0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    bool b = false;
-#pragma unroll
-                    for (int q = 0; q < QG; ++q) {
-                        float *f = reinterpret_cast<float *>(&x[k][q]);
-#pragma unroll
-                        for (int v = 0; v < 4; ++v) {
-                            if (abs_bits(f[v]) >= 0x7F800000u) {
-                                b = true;
-                                f[v] = 0.0f;
-                            }
-                            top = max(top, abs_bits(f[v]));
-                        }
-                    }
-                    if (b) vbad |= 1u << (2 * t4 + (k & 1) + (k >> 1) * 8);
-                }
-                vbad = __reduce_or_sync(0xffffffffu, vbad);
-                top = __reduce_max_sync(0xffffffffu, top);
+                    for (int q = 0; q < QG; ++q)
+                        big = max3_nan(max3_nan(big, fabsf(x[k][q].x), fabsf(x[k][q].y)), fabsf(x[k][q].z), fabsf(x[k][q].w));
+                return __reduce_max_sync(0xffffffffu, abs_bits(big));
+            };
+            uint32_t top = load();
+            if (__builtin_expect(top >= kRowsWide, 0)) {
+                vwide = settle_places(rows0, kFewUnit, hd, 0, vpe, vbad);
+                top = load();
+            }
+            const int ve = top_exp(top);
+            const float sc = pow2i(-ve);
+            if (__builtin_expect(vbad != 0, 0)) {  // the rows that see a place with a NaN or infinity become NaN
 #pragma unroll
                 for (int i = 0; i < 2 * MT; ++i)
                     if ((vbad & ~none & visible((i / 2) * 16 + g8 + (i & 1) * 8, p0)) != 0) l[i] = NAN;
             }
-            const int ve = top_exp(top);
-            const float sc = pow2i(kRowsTop - ve), osc = pow2i(ve - kRowsTop - (int)kRowsP);
+            auto values = [&](auto &&osc) {  // osc(i): what row i's products are added with
 #pragma unroll
-            for (int q = 0; q < QG; ++q) {
-                const float *f0 = reinterpret_cast<const float *>(&x[0][q]), *f1 = reinterpret_cast<const float *>(&x[1][q]),
-                            *f2 = reinterpret_cast<const float *>(&x[2][q]), *f3 = reinterpret_cast<const float *>(&x[3][q]);
+                for (int q = 0; q < QG; ++q) {
+                    const float *f0 = reinterpret_cast<const float *>(&x[0][q]), *f1 = reinterpret_cast<const float *>(&x[1][q]),
+                                *f2 = reinterpret_cast<const float *>(&x[2][q]), *f3 = reinterpret_cast<const float *>(&x[3][q]);
 #pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    float y[4] = {f0[v], f1[v], f2[v], f3[v]};
-                    if (ve != kRowsTop) y[0] *= sc, y[1] *= sc, y[2] *= sc, y[3] *= sc;
-                    uint32_t h0, h1, l0, l1;
-                    split_f16(y[0], y[1], h0, l0);
-                    split_f16(y[2], y[3], h1, l1);
+                    for (int v = 0; v < 4; ++v) {
+                        float y[4] = {f0[v], f1[v], f2[v], f3[v]};
+                        if (ve != 0) y[0] *= sc, y[1] *= sc, y[2] *= sc, y[3] *= sc;
+                        uint32_t h0, h1, l0, l1;
+                        split_f16(y[0], y[1], h0, l0);
+                        split_f16(y[2], y[3], h1, l1);
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        mma_f16(o, ph[mt], h0, h1);
-                        mma_f16(o, pl[mt], h0, h1);
-                        mma_f16(o, ph[mt], l0, l1);
+                        for (int mt = 0; mt < MT; ++mt) {
+                            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma_f16(o, ph[mt], h0, h1);
+                            mma_f16(o, pl[mt], h0, h1);
+                            mma_f16(o, ph[mt], l0, l1);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) acc[mt][4 * q + v][k] = fmaf(o[k], osc, acc[mt][4 * q + v][k]);
+                            for (int k = 0; k < 4; ++k) acc[mt][4 * q + v][k] = fmaf(o[k], osc(2 * mt + k / 2), acc[mt][4 * q + v][k]);
+                        }
                     }
                 }
+            };
+            if (__builtin_expect(!vwide, 1)) {
+                const float vsc = pow2i(ve - (int)kRowsP);
+                values([=](int) { return vsc; });
+            } else {  // P gets the places' scales relative to the row's largest weighted place
+                float rsc[2 * MT];
+                int pe[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) pe[k] = __shfl_sync(0xffffffffu, vpe, 2 * t4 + (k & 1) + (k >> 1) * 8);
+#pragma unroll
+                for (int i = 0; i < 2 * MT; ++i) {
+                    int em = -100;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) em = max(em, weight_exp(s[i / 2][k >> 1][(i & 1) * 2 + (k & 1)], pe[k]));
+                    em = max(em, __shfl_xor_sync(0xffffffffu, em, 1));
+                    em = max(em, __shfl_xor_sync(0xffffffffu, em, 2));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[i / 2][k >> 1][(i & 1) * 2 + (k & 1)] *= pow2c(pe[k] - em);
+                    rsc[i] = pow2i(em - (int)kRowsP);
+                }
+                split_p();
+                values([&](int i) { return rsc[i]; });
             }
         }
         __syncwarp();

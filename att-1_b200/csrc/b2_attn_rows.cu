@@ -30,14 +30,16 @@
 // exact): hi = f16(x 2^e), lo = f16(x 2^e - hi), and a product is
 // hi hi + lo hi + hi lo with f32 accumulation; what is dropped is below 2^-22.
 // f16 rather than bf16 pairs (2^-16) because the scale takes care of the range:
-// a row of q, eight places' K and eight places' V have a power of two each that
-// brings their largest magnitude to [1, 16), so an element 2^-9 of the largest
-// still keeps 16 bits, and what a smaller one loses is below 2^-25 of the largest.
-// (The exponents are multiples of four, so that neighbours mostly share one, and
-// mostly have none to apply.) K's scale goes
-// into the scores, V's into P relative to the tile's largest, and the tile's
-// into its O when it is summed. The softmax statistics and the weighted sums are
-// f32.
+// a row of q, eight places' K and eight places' V have a power of two each, 1 for
+// largest magnitudes from 1 to 2^12, else what brings the largest to [1, 16). So an
+// element down to 2^-9 (of the largest, where that was scaled) still keeps 16 bits,
+// and what a smaller one loses is below 2^-25. (The scaling exponents are multiples
+// of four, so that neighbours mostly share one, and mostly have none to apply.) A
+// place of 2^12 and more that is far above one of its neighbours gets its own scale,
+// as they do: a place that a row does not see, or gives no weight, takes nothing from
+// the others, whatever it holds. K's scale goes into the scores; V's into P, relative
+// to the row's largest weighted place where they differ, and that into its O when it
+// is summed. The softmax statistics and the weighted sums are f32.
 //
 // Operands in shared memory are K-major without swizzle as in b2_gemm.cu: 8-row
 // x 16-byte core matrices, row groups 128 bytes apart, 8-column chunks R * 16
@@ -48,6 +50,8 @@
 // places uses most (copies in 64 KB, conversion 64 + 64 KB, MMAs 96 KB).
 #include "b2_attn_rows.cuh"
 #include "b2_umma.cuh"
+
+#include <type_traits>
 
 namespace b2 {
 
@@ -62,7 +66,7 @@ constexpr int kRowsThreads = 32 * (kRowsSoftWarps + kRowsConvWarps + 4);  // who
 constexpr int kRowsSoftRegs = 136, kRowsConvRegs = 80, kRowsLastRegs = 40;
 static_assert(kRowsThreads == 640 && 256 * kRowsSoftRegs + 256 * kRowsConvRegs + 128 * kRowsLastRegs <= 640 * 96, "register split");
 constexpr uint32_t kRowsUnit = 16;      // places a converting warp takes of a tile
-constexpr uint32_t kRowsMeta = 8;       // ring of per-tile scales: more than the tiles between converting and softmax
+constexpr uint32_t kRowsMeta = 4;       // ring of per-tile scales: more than the tiles between converting and softmax
 
 template <int HD>
 struct RowsSmem {
@@ -76,9 +80,11 @@ struct RowsSmem {
     static constexpr uint32_t off_x = off_r + slots * slot;         // [2][2][128] f32: the halves' maxima, by tile parity
     static constexpr uint32_t off_km = off_x + 4 * kRowsM * 4;      // [kRowsMeta][8] u32: a K unit's exponent and marks
     static constexpr uint32_t off_vm = off_km + kRowsMeta * 8 * 4;  // [2][8] u32: the same of V
-    static constexpr uint32_t off_rh = off_vm + 2 * 8 * 4;          // [slots] u64: places whose page is bad
+    static constexpr uint32_t off_ke = off_vm + 2 * 8 * 4;          // [kRowsMeta][64] s8: the places' exponents of K
+    static constexpr uint32_t off_ve = off_ke + kRowsMeta * kRowsKeys;  // [2][64] s8: of V
+    static constexpr uint32_t off_rh = off_ve + 2 * kRowsKeys;      // [slots] u64: places whose page is bad
     static constexpr uint32_t off_bar = off_rh + 8 * slots;
-    static constexpr uint32_t bytes = off_bar + 8 * (2 * slots + 12) + 16;
+    static constexpr uint32_t bytes = off_bar + 8 * (2 * slots + 12) + 48;
 };
 static_assert(RowsSmem<128>::bytes <= 227 * 1024 && RowsSmem<64>::bytes <= 227 * 1024, "shared memory");
 
@@ -141,12 +147,13 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
     const uint32_t hd = EXACT ? HD : a.head_dim;  // EXACT: head_dim == HD
     float *xmax = reinterpret_cast<float *>(smem + S::off_x);
     uint32_t *kmeta = reinterpret_cast<uint32_t *>(smem + S::off_km), *vmeta = reinterpret_cast<uint32_t *>(smem + S::off_vm);
+    int8_t *kexp = reinterpret_cast<int8_t *>(smem + S::off_ke), *vexp = reinterpret_cast<int8_t *>(smem + S::off_ve);
     uint64_t *rhide = reinterpret_cast<uint64_t *>(smem + S::off_rh);
     // by parity of the tile: K and V converted, S and O computed (which frees that K and V)
     uint64_t *r_full = reinterpret_cast<uint64_t *>(smem + S::off_bar), *r_empty = r_full + NR, *k_full = r_empty + NR,
              *v_full = k_full + 2, *s_full = v_full + 2, *o_full = s_full + 2, *s_empty = o_full + 2, *p_full = s_empty + 1,
              *q_full = p_full + 1, *done = q_full + 1;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1), *met = tmem_slot + 2;  // [4][2]: the halves' meetings
 
     pdl_wait();
     pdl_launch_dependents();
@@ -180,6 +187,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
         mbar_init(p_full, nsoft);
         mbar_init(q_full, nsoft);
         mbar_init(done, 1);
+        for (uint32_t i = 0; i < 8; ++i) met[i] = 0;
         fence_mbar_init();
     }
     if (warp == kRowsMmaWarp) tmem_alloc(tmem_slot, 512);
@@ -311,59 +319,55 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
             for (uint32_t w = (warp & 3) * (kRowsUnit / 8), we = w + kRowsUnit / 8; w < we; ++w) {
                 const uint32_t place = (t0 + j) * kRowsKeys + 8 * w;
                 // places past the end (never copied) and on bad pages are zeros, hidden from every row
-                uint32_t none = (uint32_t)(hide >> (8 * w)) & 0xFFu, bad = 0;
+                const uint32_t hidden = (uint32_t)(hide >> (8 * w)) & 0xFFu;  // (the softmax knows the end itself)
+                uint32_t none = hidden, bad = 0;
                 if (place + 8 > places) none |= places <= place ? 0xFFu : (0xFFu << (places - place)) & 0xFFu;
-                const float *src = reinterpret_cast<const float *>(smem + S::off_r + sl * S::slot) + 8 * w * hd;
+                float *src = reinterpret_cast<float *>(smem + S::off_r + sl * S::slot) + 8 * w * hd;
                 float x[U];
-                uint32_t first;  // dimension of the lane's first chunk (V: of its first column)
-                if (!is_v) {
-                    // the lane's key is `key`, its chunks of eight dimensions c0, c0 + 4, ..; the rotation by
-                    // the key and the swapped halves keep the reads of eight rows and the writes of one
-                    // 16-byte column each free of bank conflicts
-                    first = 8 * c0;
-                    const float *from = src + key * hd + 8 * c0;
+                const uint32_t first = is_v ? lane : 8 * c0;  // dimension of the lane's first chunk (V: of its first column)
+                bool wide = false;
+                auto load = [&]() -> uint32_t {  // bits of the largest magnitude
+                    if (!is_v) {
+                        // the lane's key is `key`, its chunks of eight dimensions c0, c0 + 4, ..; the rotation by
+                        // the key and the swapped halves keep the reads of eight rows and the writes of one
+                        // 16-byte column each free of bank conflicts
+                        const float *from = src + key * hd + 8 * c0;
 #pragma unroll
-                    for (int k = 0; k < HD / 32; ++k) {
-                        const float *at = EXACT || 32 * k + 8 * c0 < hd ? from + 32 * k : from - 8 * c0;
-                        const float4 f = *reinterpret_cast<const float4 *>(at + swap), g = *reinterpret_cast<const float4 *>(at + (swap ^ 4));
-                        x[8 * k] = swap ? g.x : f.x, x[8 * k + 1] = swap ? g.y : f.y, x[8 * k + 2] = swap ? g.z : f.z,
-                        x[8 * k + 3] = swap ? g.w : f.w, x[8 * k + 4] = swap ? f.x : g.x, x[8 * k + 5] = swap ? f.y : g.y,
-                        x[8 * k + 6] = swap ? f.z : g.z, x[8 * k + 7] = swap ? f.w : g.w;
-                    }
-                } else {
-                    // dimensions lane + 32 k of the eight places
-                    first = lane;
-#pragma unroll
-                    for (int c = 0; c < 8; ++c)
-#pragma unroll
-                        for (int k = 0; k < HD / 32; ++k)
-                            x[8 * k + c] = src[c * hd + (EXACT || lane + 32 * k < hd ? lane + 32 * k : 0)];
-                }
-                if (none != 0) {
-#pragma unroll
-                    for (int k = 0; k < U; ++k)
-                        if (none >> (is_v ? k & 7 : key) & 1) x[k] = 0.0f;
-                }
-                float big = 0.0f;
-#pragma unroll
-                for (int k = 0; k < U; k += 2) big = max3_nan(big, fabsf(x[k]), fabsf(x[k + 1]));
-                uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(big));  // a NaN's bits are above infinity's
-                if (top >= 0x7F800000u) {  // a NaN or infinity: zero it, mark its place
-                    top = 0;
-#pragma unroll
-                    for (int k = 0; k < U; ++k) {
-                        if (abs_bits(x[k]) >= 0x7F800000u) {
-                            bad |= 1u << (is_v ? k & 7 : key);
-                            x[k] = 0.0f;
+                        for (int k = 0; k < HD / 32; ++k) {
+                            const float *at = EXACT || 32 * k + 8 * c0 < hd ? from + 32 * k : from - 8 * c0;
+                            const float4 f = *reinterpret_cast<const float4 *>(at + swap), g = *reinterpret_cast<const float4 *>(at + (swap ^ 4));
+                            x[8 * k] = swap ? g.x : f.x, x[8 * k + 1] = swap ? g.y : f.y, x[8 * k + 2] = swap ? g.z : f.z,
+                            x[8 * k + 3] = swap ? g.w : f.w, x[8 * k + 4] = swap ? f.x : g.x, x[8 * k + 5] = swap ? f.y : g.y,
+                            x[8 * k + 6] = swap ? f.z : g.z, x[8 * k + 7] = swap ? f.w : g.w;
                         }
-                        top = max(top, abs_bits(x[k]));
+                    } else {
+                        // dimensions lane + 32 k of the eight places
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+#pragma unroll
+                            for (int k = 0; k < HD / 32; ++k)
+                                x[8 * k + c] = src[c * hd + (EXACT || lane + 32 * k < hd ? lane + 32 * k : 0)];
                     }
-                    top = __reduce_max_sync(0xffffffffu, top);
-                    bad = __reduce_or_sync(0xffffffffu, bad);
+                    if (none != 0) {
+#pragma unroll
+                        for (int k = 0; k < U; ++k)
+                            if (none >> (is_v ? k & 7 : key) & 1) x[k] = 0.0f;
+                    }
+                    float big = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < U; k += 2) big = max3_nan(big, fabsf(x[k]), fabsf(x[k + 1]));
+                    return __reduce_max_sync(0xffffffffu, abs_bits(big));  // a NaN's bits are above infinity's
+                };
+                uint32_t top = load();
+                if (__builtin_expect(top >= kRowsWide, 0)) {
+                    int pe;
+                    wide = settle_places(src, 8, hd, none, pe, bad);
+                    if (wide && lane < 8) (is_v ? vexp + st * kRowsKeys : kexp + (j % kRowsMeta) * kRowsKeys)[8 * w + lane] = (int8_t)pe;
+                    top = load();
                 }
                 const int e = top_exp(top);
-                if (e != kRowsTop) {
-                    const float sc = pow2i(kRowsTop - e);
+                if (e != 0) {
+                    const float sc = pow2i(-e);
                     const uint64_t sc2 = pair(sc, sc);
 #pragma unroll
                     for (int k = 0; k < U; k += 2) unpair(mul2(pair(x[k], x[k + 1]), sc2), x[k], x[k + 1]);
@@ -384,7 +388,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                         *reinterpret_cast<uint4 *>(dst + k * step + to_lo) = l;
                     }
                 }
-                if (lane == 0) (is_v ? vmeta + st * 8 : kmeta + (j % kRowsMeta) * 8)[w] = unit_meta(e, none, bad);
+                if (lane == 0) (is_v ? vmeta + st * 8 : kmeta + (j % kRowsMeta) * 8)[w] = unit_meta(e, wide, hidden, bad);
             }
             fence_proxy_async();
             __syncwarp();
@@ -412,8 +416,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 }
                 const bool bad = top >= 0x7F800000u;
                 const int e = bad ? 0 : top_exp(top);
-                const float sc = pow2i(kRowsTop - e);
-                cq = bad ? NAN : pow2i(e - kRowsTop) * p.scale;
+                const float sc = pow2i(-e);
+                cq = bad ? NAN : pow2i(e) * p.scale;
 #pragma unroll
                 for (uint32_t c = 0; c < HD / 2; c += 32) {  // 32 dimensions: 16 columns of hi, 16 of lo
                     uint32_t hi[16], lo[16];
@@ -443,6 +447,21 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
             bool ok = true;
             auto wait = [&](uint64_t *bar, uint32_t phase) { ok = ok && warp_wait(bar, phase, a.err); };
             auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + qt) : "memory"); };
+            // Where only some tiles meet: want grows from meeting to meeting, and it ends by itself
+            // even if one of the two never comes.
+            auto meet_again = [&](uint32_t want) {
+                volatile uint32_t *at = met + 2 * qt;
+                __threadfence_block();
+                __syncwarp();
+                at[half] = want;
+                for (uint32_t i = 0; ok && at[half ^ 1] < want; ++i) ok = i < (1u << 22);
+                ok = __all_sync(0xffffffffu, ok);
+                __threadfence_block();
+            };
+            // exponent of a place of a tile
+            auto exp_of = [&](const uint32_t *unit, const int8_t *place, uint32_t k) -> int {
+                return unit[k / 8] >> 24 ? (int)place[k] : meta_exp(unit[k / 8]);
+            };
             // O of the tile before into the sums: acc = acc * corr + O * osc
             auto take_o = [&]() {
                 const uint32_t col = tm_o + lanes + half * (HD / 2);
@@ -482,14 +501,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 if (key0 + 32 > places) vis &= places <= key0 ? 0 : (1u << (places - key0)) - 1;
                 return vis;
             };
-            for (uint32_t j = 0; j < nt; ++j) {
+            // One tile. Units of K or V of different scale and marked places are rare and cost the
+            // others nothing: they have a copy of the code of their own (in one, the branches and
+            // what they keep in registers slowed every tile by 5 to 9 percent).
+            auto tile = [&](uint32_t j, auto rare, const uint4 &km, const uint4 &va, const uint4 &vb) {
+                constexpr bool RARE = decltype(rare)::value;
                 const uint32_t mt = j % kRowsMeta, vt = j & 1, key0 = (t0 + j) * kRowsKeys + half * 32;
-                wait(&s_full[j & 1], j / 2);
-                tc_fence_after();
                 uint32_t raw[32], low[16];
                 tmem_ld32(tm_s + lanes + half * 32, raw);
                 tmem_ld16_nowait(tm_s + lanes + kRowsKeys + half * 32, low);
-                const uint4 km = *reinterpret_cast<const uint4 *>(kmeta + mt * 8 + half * 4);
                 float s[32];
                 tmem_wait_ld();
                 auto sum16 = [&](int k0) {
@@ -506,18 +526,17 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_empty);
                 sum16(16);
-                int ks = meta_exp(km.x);
+                float cqk = cq * pow2i(meta_exp(km.x));
                 uint32_t vis = key0 + 32 > ctx ? visible(key0) : 0xFFFFFFFFu;
-                if (!meta_plain(km)) {  // units of different scale, places hidden or not finite
-                    const int eu[4] = {ks, meta_exp(km.y), meta_exp(km.z), meta_exp(km.w)};
-                    ks = max(max(eu[0], eu[1]), max(eu[2], eu[3]));
+                if (RARE && !meta_plain(km)) {
                     const uint32_t bad = meta_bytes(km, 0);
                     vis &= ~meta_bytes(km, 8);
 #pragma unroll
                     for (int k = 0; k < 32; ++k) {
-                        s[k] *= pow2i(max(eu[k / 8] - ks, -126));
+                        s[k] = s[k] * cq * pow2i(exp_of(kmeta + mt * 8, kexp + mt * kRowsKeys, half * 32 + k));
                         if (bad >> k & 1) s[k] = NAN;
                     }
+                    cqk = 1.0f;
                 }
                 if (vis != 0xFFFFFFFFu) {
 #pragma unroll
@@ -531,7 +550,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                     top2 = max3(top2, s[k + 2], s[k + 3]);
                 }
                 top = fmaxf(top, top2);
-                const float cqk = cq * pow2i(ks - kRowsTop);
                 // the row's maximum over both halves
                 float *x = xmax + (j & 1) * 2 * kRowsM;
                 x[half * kRowsM + r] = top * cqk;
@@ -555,16 +573,21 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 float sy, sz;
                 unpair(sum, sy, sz);
                 l = fmaf(l, corr, sy + sz);
-                wait(&v_full[vt], j / 2);
-                const uint4 va = *reinterpret_cast<const uint4 *>(vmeta + vt * 8), vb = *reinterpret_cast<const uint4 *>(vmeta + vt * 8 + 4);
                 int emax = meta_exp(va.x);
-                if (!meta_plain(va) || !meta_plain(vb) || va.x != vb.x) {  // units of different scale, or a NaN or infinity in V
-                    emax = max(max(max(emax, meta_exp(va.y)), max(meta_exp(va.z), meta_exp(va.w))),
-                               max(max(meta_exp(vb.x), meta_exp(vb.y)), max(meta_exp(vb.z), meta_exp(vb.w))));
+                if (RARE && !(meta_plain(va) && meta_plain(vb) && va.x == vb.x)) {
+                    // P takes V's scales relative to the row's own largest weighted place
                     const uint4 vh = half ? vb : va;
-                    const int eu[4] = {meta_exp(vh.x), meta_exp(vh.y), meta_exp(vh.z), meta_exp(vh.w)};
+                    const uint32_t *mu = vmeta + vt * 8;
+                    const int8_t *pe = vexp + vt * kRowsKeys;
+                    emax = -100;
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) s[k] *= pow2i(max(eu[k / 8] - emax, -126));
+                    for (int k = 0; k < 32; ++k) emax = max(emax, weight_exp(s[k], exp_of(mu, pe, half * 32 + k)));
+                    meet_again(2 * j + 1);  // both have read the maxima
+                    x[half * kRowsM + r] = __int_as_float(emax);
+                    meet_again(2 * j + 2);
+                    emax = max(emax, __float_as_int(x[(half ^ 1) * kRowsM + r]));
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) s[k] *= pow2c(exp_of(mu, pe, half * 32 + k) - emax);
                     if ((meta_bytes(vh, 0) & visible(key0)) != 0) l = NAN;
                 }
                 uint32_t hi[16], lo[16];
@@ -580,7 +603,16 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full);
                 corr_prev = corr;
-                osc_prev = pow2i(emax - kRowsTop - (int)kRowsP);
+                osc_prev = pow2i(emax - (int)kRowsP);
+            };
+            for (uint32_t j = 0; j < nt; ++j) {
+                wait(&s_full[j & 1], j / 2);
+                wait(&v_full[j & 1], j / 2);
+                tc_fence_after();
+                const uint4 km = *reinterpret_cast<const uint4 *>(kmeta + (j % kRowsMeta) * 8 + half * 4),
+                            va = *reinterpret_cast<const uint4 *>(vmeta + (j & 1) * 8), vb = *reinterpret_cast<const uint4 *>(vmeta + (j & 1) * 8 + 4);
+                if (meta_plain(km) && meta_plain(va) && meta_plain(vb) && va.x == vb.x) tile(j, std::false_type(), km, va, vb);
+                else tile(j, std::true_type(), km, va, vb);
             }
             wait(&o_full[(nt - 1) & 1], (nt - 1) / 2);
             tc_fence_after();
@@ -596,6 +628,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 unpair(acc[c / 2 + 1], f.z, f.w);
                 return f;
             };
+            if (!ok && lane == 0) raise_error(a.err, B2_ERR_TIMEOUT);
             if (ok && mine) {
                 // the weights carry 2^11, the sums of O do not
                 const float lw = l * pow2i(-(int)kRowsP);

@@ -9,7 +9,6 @@
 
 namespace b2 {
 
-constexpr int kRowsTop = 0;             // operands are scaled to [2^kRowsTop, 2^(kRowsTop + 4))
 constexpr float kRowsP = 11.0f;         // P is scaled by 2^11,
 constexpr float kRowsSlack = 4.0f;      // and may pass that by 2^4 (f16 ends at 2^16) before the maximum is raised
 constexpr uint32_t kRowsMaxSplits = 64;
@@ -63,11 +62,19 @@ __device__ __forceinline__ float ex2(float x)
     return y;
 }
 
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126..127
 
-// Exponent of the largest magnitude (its bits), down to a multiple of four and
-// floored so that the scale 2^(kRowsTop - e) and its inverse stay normal.
-__device__ __forceinline__ int top_exp(uint32_t amax_bits) { return max(((int)(amax_bits >> 23) - 127) & ~3, -100); }
+// The exponent e that operands of this largest magnitude (its bits) are scaled by, as
+// x 2^-e: 0 from 2^-4 up to 2^12 and for zeros, else what brings it to [1, 16), floored so
+// that 2^-e stays normal.
+__device__ __forceinline__ int top_exp(uint32_t amax_bits)
+{
+    const int e = (int)(amax_bits >> 23) - 127;
+    return (uint32_t)(e + 4) < 16u || amax_bits == 0 ? 0 : max(e & ~3, -100);
+}
+constexpr uint32_t kRowsWide = 139u << 23;  // bits of 2^12
 
 // Two f32 in one register pair.
 __device__ __forceinline__ uint64_t pair(float a, float b)
@@ -120,17 +127,67 @@ __device__ __forceinline__ void cut_f16(float a, float b, uint32_t &hi, uint32_t
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
-// What the softmax needs to know of a unit: exponent, places hidden from every
-// row, places with a NaN or infinity.
-__device__ __forceinline__ uint32_t unit_meta(int e, uint32_t hidden, uint32_t bad) { return (uint32_t)(e + 128) << 16 | hidden << 8 | bad; }
-__device__ __forceinline__ int meta_exp(uint32_t m) { return (int)(m >> 16) - 128; }
+// What the softmax needs to know of a unit: exponent, whether its places have their
+// own, places hidden from every row, places with a NaN or infinity.
+__device__ __forceinline__ uint32_t unit_meta(int e, bool wide, uint32_t hidden, uint32_t bad)
+{
+    return (uint32_t)wide << 24 | (uint32_t)(e + 128) << 16 | hidden << 8 | bad;
+}
+__device__ __forceinline__ int meta_exp(uint32_t m) { return (int)(m >> 16 & 0xFF) - 128; }
 // byte i of the result: (m_i >> shift) & 0xFF
 __device__ __forceinline__ uint32_t meta_bytes(const uint4 &m, uint32_t shift)
 {
     return (m.x >> shift & 0xFF) | (m.y >> shift & 0xFF) << 8 | (m.z >> shift & 0xFF) << 16 | (m.w >> shift & 0xFF) << 24;
 }
 // Four units that share an exponent and have nothing marked.
-__device__ __forceinline__ bool meta_plain(const uint4 &m) { return m.x == m.y && m.x == m.z && m.x == m.w && (m.x & 0xFFFF) == 0; }
+__device__ __forceinline__ bool meta_plain(const uint4 &m) { return m.x == m.y && m.x == m.z && m.x == m.w && (m.x & 0x100FFFF) == 0; }
+
+// Places that share an exponent e lose what is below 2^-25 of the largest (of 1, if that
+// is between 1 and 2^12). A larger place that few rows see, or that has next to no weight,
+// must not take that from its neighbours: among places of 2^12 and more, each has its own
+// exponent if one is kRowsSpread or more below another.
+// rows: `places` rows of hd values in shared memory, all a warp's; bits of none: rows that
+// are not there. Zeroes NaNs and infinities (bits of bad), and if it returns true has scaled
+// row i by 2^-pe of lane i.
+constexpr int kRowsSpread = 8;
+__device__ __forceinline__ bool settle_places(float *rows, uint32_t places, uint32_t hd, uint32_t none, int &pe, uint32_t &bad)
+{
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t mine = 0;
+#pragma unroll 1
+    for (uint32_t c = 0; c < places; ++c) {
+        uint32_t top = 0;
+        bool b = false;
+#pragma unroll 1
+        for (uint32_t d = none >> c & 1 ? hd : lane; d < hd; d += 32) {
+            const uint32_t v = abs_bits(rows[c * hd + d]);
+            if (v < 0x7F800000u) {
+                top = max(top, v);
+            } else {
+                b = true;
+                rows[c * hd + d] = 0.0f;
+            }
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (__any_sync(0xffffffffu, b)) bad |= 1u << c;
+        if (lane == c) mine = top;
+    }
+    const int e = top_exp(__reduce_max_sync(0xffffffffu, mine));
+    pe = mine == 0 ? e : top_exp(mine);
+    const bool wide = __any_sync(0xffffffffu, pe <= e - kRowsSpread) && e > 0;
+#pragma unroll 1
+    for (uint32_t c = 0; wide && c < places; ++c) {
+        const float sc = pow2i(-__shfl_sync(0xffffffffu, pe, c));
+#pragma unroll 1
+        for (uint32_t d = none >> c & 1 ? hd : lane; d < hd; d += 32) rows[c * hd + d] *= sc;
+    }
+    __syncwarp();
+    return wide;
+}
+// Exponent of a weighted place, p 2^e, with p (times 2^kRowsP) at most 1.
+__device__ __forceinline__ int weight_exp(float p, int e) { return p > 0.0f ? e + ((int)(__float_as_uint(p) >> 23) - 127) - (int)kRowsP : -100; }
+__device__ __forceinline__ float pow2c(int e) { return pow2i(min(max(e, -126), 127)); }
+
 
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
@@ -145,8 +202,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c)
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
 // All lanes wait; false for the whole warp if any gave up.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase, int32_t *err)

@@ -237,6 +237,65 @@ def test_attn_masked_places_may_hold_anything(b2, torch):
             assert err == ERR_NONFINITE
 
 
+@pytest.mark.parametrize("big", [3e3, 1e10, 1e30, 3e38])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("h,hkv,hd,new,victim", [(4, 2, 64, 10, 6), (2, 1, 128, 16, 3), (8, 2, 128, 24, 17), (4, 1, 64, 40, 9)])
+def test_attn_hidden_place_takes_no_precision(b2, torch, h, hkv, hd, new, victim, which, big):
+    """A finite K or V of any size in a drafted row: the rows that do not see it keep their error bound."""
+    s = Scene(torch, h, hkv, hd, 16, [37], [new], seed=13)
+    ref = s.reference()
+    pg, off = s.place(0, 37 + victim)
+    getattr(s, which)[pg, :, off] = big * np.sign(getattr(s, which)[pg, :, off])
+    got, err = s.run(b2)
+    for i in range(new):
+        if not s.masks[i] >> victim & 1:
+            assert np.abs(got[i] - ref[i]).max() <= ATTN_TOL * 5
+
+
+@pytest.mark.parametrize("h,hkv,hd,new", [(4, 2, 64, 10), (8, 2, 128, 24)])
+@pytest.mark.parametrize("at", [5, 20, 36])
+def test_attn_place_of_no_weight_takes_no_precision(b2, torch, h, hkv, hd, new, at):
+    """A cached place whose K is 2^14 times the others' in one direction: rows it draws to itself give its V,
+    the others do as if it were not there, also where its V is 2^40."""
+    s = Scene(torch, h, hkv, hd, 16, [37], [new], seed=16)
+    pg, off = s.place(0, at)
+    s.k[pg, :, off] = 0
+    s.k[pg, :, off, 3] = 2.0 ** 14
+    s.v[pg, :, off] = 2.0 ** 40
+    q = s.q[:s.rows, :h * hd].reshape(s.rows, h, hd)
+    q[:, :, 3] = np.where(q[:, :, 3] > 0, 1, -1)  # scores of +-2^14 / sqrt(hd)
+    got, err = s.run(b2)
+    assert err == 0
+    drawn = q[:, :, 3] > 0
+    assert drawn.any() and not drawn.all()
+    assert (np.abs(got[drawn] - 2.0 ** 40) <= ATTN_TOL * 2.0 ** 40).all()
+    t = 37 + new
+    pages, offs = s.table[0, np.arange(t) // 16], np.arange(t) % 16
+    for i in range(new):
+        seen = [x for x in s.sees(0, i) if x != at]
+        for hh in range(h):
+            if drawn[i, hh]:
+                continue
+            K = s.k[pages[seen], hh // (h // hkv), offs[seen]].astype(np.float64)
+            V = s.v[pages[seen], hh // (h // hkv), offs[seen]].astype(np.float64)
+            w = np.exp((sc := K @ q[i, hh].astype(np.float64) / np.sqrt(hd)) - sc.max())
+            assert np.abs(got[i, hh] - w @ V / w.sum()).max() <= ATTN_TOL * 5
+
+
+@pytest.mark.parametrize("h,hkv,hd,new", [(4, 2, 64, 10), (2, 1, 128, 16), (8, 2, 128, 40), (4, 1, 48, 64)])
+def test_attn_values_of_mixed_sizes(b2, torch, h, hkv, hd, new):
+    """Every place's V times a power of two of its own, 2^-14 to 2^14."""
+    s = Scene(torch, h, hkv, hd, 16, [150], [new], seed=18)
+    s.v *= np.ldexp(np.float32(1), np.random.default_rng(7).integers(-14, 15, s.v.shape[0] * 16)).reshape(-1, 1, 16, 1).astype(np.float32)
+    got, err = s.run(b2)
+    assert err == 0
+    ref, v = s.reference(), s.v
+    s.v = np.abs(v)
+    size = s.reference()  # sum_j p_j |v_j|, per dimension
+    # a product keeps 2^-22 of itself, an element of V 2^-25 of 1 besides (where no place of 2^12 is near)
+    assert (np.abs(got - ref) <= ATTN_TOL * size.max(-1, keepdims=True) + 2.0 ** -24).all()
+
+
 def test_attn_nonfinite_query(b2, torch):
     s = Scene(torch, 4, 2, 64, 16, [37], [5], seed=14)
     ref = s.reference()
