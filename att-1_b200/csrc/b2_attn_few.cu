@@ -1,5 +1,5 @@
 // b2_attn_few.cu - attention of a few new rows per sequence over the paged KV cache:
-// b2_attn_rows for up to 32 rows (tokens x query heads of a KV head). Same arithmetic
+// b2_attn_rows for up to 16 rows (tokens x query heads of a KV head). Same arithmetic
 // as b2_attn_rows.cu: every f32 operand as two f16 numbers of a power-of-two multiple,
 // three products, f32 sums.
 //
@@ -18,13 +18,15 @@
 //   to the f32 sums with the 16 places' scale, so no sum runs through more than three
 //   MMAs of O, or 3 head_dim / 16 of S.
 // A lane holds the softmax statistics of its rows; the warps' sums are joined in shared
-// memory in warp order, then the splits' in split order: up to eight are a cluster and
-// read each other's shared memory, more go to attn_rows_join_kernel.
+// memory in warp order, then the splits' in split order: up to eight, a cluster whose CTAs
+// read each other's shared memory.
 #include "b2_attn_rows.cuh"
 
 namespace b2 {
 
-template <int HD, int MT>
+constexpr int MT = kFewRows / 16;  // MMA tiles of rows
+
+template <int HD>
 struct FewSmem {
     static constexpr uint32_t slots = HD == 128 ? 3 : 6;          // per warp
     static constexpr uint32_t slot = kFewUnit * HD * 4;
@@ -46,12 +48,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint4 &a, uint32_t 
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
-}
-
-// 16 bytes global to shared, or zeros (from 0).
-__device__ __forceinline__ void cp_async16(void *dst, const void *src, uint32_t from)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(from) : "memory");
 }
 
 // All threads of the cluster; what was written to shared memory before is seen after.
@@ -79,10 +75,10 @@ __device__ __forceinline__ float4 cluster_ld4(const void *p, uint32_t rank)
     return v;
 }
 
-template <int HD, int MT>
+template <int HD>
 __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsParams p)
 {
-    using S = FewSmem<HD, MT>;
+    using S = FewSmem<HD>;
     constexpr uint32_t NS = S::slots;
     constexpr int KS = HD / 16, QG = HD / 32;  // 16-dimension steps; groups of 32 dimensions
     extern __shared__ __align__(128) uint8_t smem[];
@@ -105,7 +101,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
     const uint32_t places = rows_places(p, n, ctx, 0);
     uint32_t t0, t1;
     rows_range(p, places, split, t0, t1);
-    if (t0 == t1 && !p.cluster) return;  // (a cluster's CTAs meet at its end)
     const uint32_t nc = t1 - t0 > warp ? (t1 - t0 - warp + kFewWarps - 1) / kFewWarps : 0;  // this warp's units
 
     // ---- the ring: unit c of this warp is K in fill 2 c, V in fill 2 c + 1 ----
@@ -289,7 +284,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
         fill();  // into the slot just read
         // ---- softmax: a lane holds columns 8 nt + 2 t4, + 1 of its rows ----
         const bool masked = p0 + kFewUnit > ctx || none != 0 || kbad != 0;
-        const float kf = pow2i(ke);
         if (__builtin_expect(kwide, 0)) {
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt)
@@ -305,7 +299,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i) {
             float *s0 = &s[i / 2][0][(i & 1) * 2], *s1 = &s[i / 2][1][(i & 1) * 2];
-            const float cqk = kwide ? 1.0f : cq[i] * kf;
+            const float cqk = kwide ? 1.0f : score_factor(cq[i], ke);
             if (masked) {
                 const uint32_t vis = visible((i / 2) * 16 + g8 + (i & 1) * 8, p0) & ~none;
 #pragma unroll
@@ -481,18 +475,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
             L = fmaf(ml.y, f, L);
             o = make_float4(fmaf(x.x, f, o.x), fmaf(x.y, f, o.y), fmaf(x.z, f, o.z), fmaf(x.w, f, o.w));
         }
-        if (p.cluster) {
+        if (p.splits > 1) {
             *reinterpret_cast<float4 *>(O0 + (size_t)r * HD + d) = o;
             if (d == 0) ML[kFewWarps * 16 * MT + r] = make_float2(M, L);
-        } else if (p.splits > 1) {
-            float *dst = rows_part(p, item, kvh, 0, split) + (size_t)r * (hd + 4);
-            if (d == 0) *reinterpret_cast<float2 *>(dst) = make_float2(M, L);
-            *reinterpret_cast<float4 *>(dst + 4 + d) = o;
         } else {
             finish(r, d, L, o);
         }
     }
-    if (!p.cluster) return;
+    if (p.splits == 1) return;
     cluster_sync();
     for (uint32_t i = split * kFewWarps * 32 + threadIdx.x; i < rows * (HD / 4); i += p.splits * kFewWarps * 32) {
         const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
@@ -524,15 +514,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
     cluster_sync();  // no CTA ends while another reads its sums
 }
 
-template <int HD, int MT>
+template <int HD>
 static cudaError_t launch_few(const RowsParams &p, cudaStream_t st)
 {
-    const cudaError_t e = cudaFuncSetAttribute(attn_few_kernel<HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FewSmem<HD, MT>::bytes);
+    const cudaError_t e = cudaFuncSetAttribute(attn_few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FewSmem<HD>::bytes);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.splits, p.a.n_kv_heads, p.a.batch);
     cfg.blockDim = dim3(kFewWarps * 32);
-    cfg.dynamicSmemBytes = FewSmem<HD, MT>::bytes;
+    cfg.dynamicSmemBytes = FewSmem<HD>::bytes;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -541,14 +531,13 @@ static cudaError_t launch_few(const RowsParams &p, cudaStream_t st)
     attr[1].val.clusterDim.x = p.splits;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = p.cluster ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, attn_few_kernel<HD, MT>, p);
+    cfg.numAttrs = p.splits > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, attn_few_kernel<HD>, p);
 }
 
 cudaError_t attn_few_launch(const RowsParams &p, cudaStream_t st)
 {
-    if (p.a.head_dim > 64) return p.block == 16 ? launch_few<128, 1>(p, st) : launch_few<128, 2>(p, st);
-    return p.block == 16 ? launch_few<64, 1>(p, st) : launch_few<64, 2>(p, st);
+    return p.a.head_dim > 64 ? launch_few<128>(p, st) : launch_few<64>(p, st);
 }
 
 }  // namespace b2

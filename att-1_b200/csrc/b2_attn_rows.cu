@@ -55,8 +55,6 @@
 
 namespace b2 {
 
-constexpr uint32_t kRowsM = 128;        // (token, query head) rows of a CTA
-constexpr uint32_t kRowsKeys = 64;      // places of a tile
 constexpr int kRowsSoftWarps = 8;
 constexpr int kRowsConvWarps = 8;
 constexpr uint32_t kRowsMmaWarp = kRowsSoftWarps + kRowsConvWarps, kRowsCopyWarp = kRowsMmaWarp + 1;
@@ -65,7 +63,6 @@ constexpr int kRowsThreads = 32 * (kRowsSoftWarps + kRowsConvWarps + 4);  // who
 // the last one; the launch gives every thread 96 (five warps per scheduler).
 constexpr int kRowsSoftRegs = 136, kRowsConvRegs = 80, kRowsLastRegs = 40;
 static_assert(kRowsThreads == 640 && 256 * kRowsSoftRegs + 256 * kRowsConvRegs + 128 * kRowsLastRegs <= 640 * 96, "register split");
-constexpr uint32_t kRowsUnit = 16;      // places a converting warp takes of a tile
 constexpr uint32_t kRowsMeta = 4;       // ring of per-tile scales: more than the tiles between converting and softmax
 
 template <int HD>
@@ -87,53 +84,6 @@ struct RowsSmem {
     static constexpr uint32_t bytes = off_bar + 8 * (2 * slots + 12) + 48;
 };
 static_assert(RowsSmem<128>::bytes <= 227 * 1024 && RowsSmem<64>::bytes <= 227 * 1024, "shared memory");
-
-// 32 lanes x 32 columns: thread i gets lane (base + i), columns col..col+31. The
-// registers hold after tmem_wait_ld.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
-{
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                 : "r"(taddr)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16])
-{
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16])
-{
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// mbar_wait_bounded of one thread without the suspension of mbar_try_wait.
-__device__ __forceinline__ bool spin_wait(uint64_t *bar, uint32_t parity, int32_t *err)
-{
-    for (uint32_t i = 0; i < (1u << 26); ++i) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity)
-            : "memory");
-        if (ok) return true;
-    }
-    raise_error(err, B2_ERR_TIMEOUT);
-    return false;
-}
 
 template <int HD, bool EXACT>
 __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsParams p)
@@ -255,7 +205,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
             if (fault) raise_error(a.err, fault);
         } else if (warp == kRowsMmaWarp) {
             // ---- MMA issue ----
-            if (lane == 0) {
+            if (elect_one()) {
                 const uint32_t id_s2 = umma_idesc_f16(kRowsM, 2 * kRowsKeys), id_s = umma_idesc_f16(kRowsM, kRowsKeys),
                            id_o = umma_idesc_f16(kRowsM, hd);
                 const uint32_t kb = smem_u32(smem + S::off_k), vb = smem_u32(smem + S::off_v);
@@ -306,8 +256,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
         // values; the conversion of its HD / 32 chunks of eight (16 bytes of hi, 16 of lo) is
         // one piece of code for both: the roles of this kernel run different code side by
         // side, and instruction fetch is what they run out of first.
-        constexpr int U = HD / 4;  // values a lane holds of eight places
-        const uint32_t key = lane & 7, c0 = ((lane >> 3) + key) & 3, swap = key & 4;
         const bool is_v = warp >= (uint32_t)kRowsSoftWarps + 4;
         for (uint32_t j = 0; j < nt; ++j) {
             const uint32_t i = 2 * j + is_v, sl = i % NR;
@@ -320,75 +268,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 const uint32_t place = (t0 + j) * kRowsKeys + 8 * w;
                 // places past the end (never copied) and on bad pages are zeros, hidden from every row
                 const uint32_t hidden = (uint32_t)(hide >> (8 * w)) & 0xFFu;  // (the softmax knows the end itself)
-                uint32_t none = hidden, bad = 0;
+                uint32_t none = hidden;
                 if (place + 8 > places) none |= places <= place ? 0xFFu : (0xFFu << (places - place)) & 0xFFu;
-                float *src = reinterpret_cast<float *>(smem + S::off_r + sl * S::slot) + 8 * w * hd;
-                float x[U];
-                const uint32_t first = is_v ? lane : 8 * c0;  // dimension of the lane's first chunk (V: of its first column)
-                bool wide = false;
-                auto load = [&]() -> uint32_t {  // bits of the largest magnitude
-                    if (!is_v) {
-                        // the lane's key is `key`, its chunks of eight dimensions c0, c0 + 4, ..; the rotation by
-                        // the key and the swapped halves keep the reads of eight rows and the writes of one
-                        // 16-byte column each free of bank conflicts
-                        const float *from = src + key * hd + 8 * c0;
-#pragma unroll
-                        for (int k = 0; k < HD / 32; ++k) {
-                            const float *at = EXACT || 32 * k + 8 * c0 < hd ? from + 32 * k : from - 8 * c0;
-                            const float4 f = *reinterpret_cast<const float4 *>(at + swap), g = *reinterpret_cast<const float4 *>(at + (swap ^ 4));
-                            x[8 * k] = swap ? g.x : f.x, x[8 * k + 1] = swap ? g.y : f.y, x[8 * k + 2] = swap ? g.z : f.z,
-                            x[8 * k + 3] = swap ? g.w : f.w, x[8 * k + 4] = swap ? f.x : g.x, x[8 * k + 5] = swap ? f.y : g.y,
-                            x[8 * k + 6] = swap ? f.z : g.z, x[8 * k + 7] = swap ? f.w : g.w;
-                        }
-                    } else {
-                        // dimensions lane + 32 k of the eight places
-#pragma unroll
-                        for (int c = 0; c < 8; ++c)
-#pragma unroll
-                            for (int k = 0; k < HD / 32; ++k)
-                                x[8 * k + c] = src[c * hd + (EXACT || lane + 32 * k < hd ? lane + 32 * k : 0)];
-                    }
-                    if (none != 0) {
-#pragma unroll
-                        for (int k = 0; k < U; ++k)
-                            if (none >> (is_v ? k & 7 : key) & 1) x[k] = 0.0f;
-                    }
-                    float big = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < U; k += 2) big = max3_nan(big, fabsf(x[k]), fabsf(x[k + 1]));
-                    return __reduce_max_sync(0xffffffffu, abs_bits(big));  // a NaN's bits are above infinity's
-                };
-                uint32_t top = load();
-                if (__builtin_expect(top >= kRowsWide, 0)) {
-                    int pe;
-                    wide = settle_places(src, 8, hd, none, pe, bad);
-                    if (wide && lane < 8) (is_v ? vexp + st * kRowsKeys : kexp + (j % kRowsMeta) * kRowsKeys)[8 * w + lane] = (int8_t)pe;
-                    top = load();
-                }
-                const int e = top_exp(top);
-                if (e != 0) {
-                    const float sc = pow2i(-e);
-                    const uint64_t sc2 = pair(sc, sc);
-#pragma unroll
-                    for (int k = 0; k < U; k += 2) unpair(mul2(pair(x[k], x[k + 1]), sc2), x[k], x[k + 1]);
-                }
-                // element (key, d) of K: chunk d / 8 of 128 rows (64 hi, 64 lo); (d, place) of V: chunk place / 8 of HD rows
-                uint8_t *dst = smem + (is_v ? S::off_v + st * 2 * S::half + w * (HD * 16) + lane * 16
-                                            : S::off_k + st * 2 * S::half + c0 * (2 * kRowsKeys * 16) + w * 128 + key * 16);
-                const uint32_t step = is_v ? 32 * 16 : 4 * (2 * kRowsKeys * 16), to_lo = is_v ? S::half : kRowsKeys * 16;
-#pragma unroll
-                for (uint32_t k = 0; k < HD / 32; ++k) {
-                    if (EXACT || first + 32 * k < hd) {
-                        uint4 h, l;
-                        split_f16(x[8 * k], x[8 * k + 1], h.x, l.x);
-                        split_f16(x[8 * k + 2], x[8 * k + 3], h.y, l.y);
-                        split_f16(x[8 * k + 4], x[8 * k + 5], h.z, l.z);
-                        split_f16(x[8 * k + 6], x[8 * k + 7], h.w, l.w);
-                        *reinterpret_cast<uint4 *>(dst + k * step) = h;
-                        *reinterpret_cast<uint4 *>(dst + k * step + to_lo) = l;
-                    }
-                }
-                if (lane == 0) (is_v ? vmeta + st * 8 : kmeta + (j % kRowsMeta) * 8)[w] = unit_meta(e, wide, hidden, bad);
+                const uint32_t m = lay_unit<HD, EXACT>(reinterpret_cast<float *>(smem + S::off_r + sl * S::slot) + 8 * w * hd, hd, is_v, w, none, hidden,
+                                                       smem + (is_v ? S::off_v : S::off_k) + st * 2 * S::half, kRowsKeys * 16,
+                                                       is_v ? vexp + st * kRowsKeys : kexp + (j % kRowsMeta) * kRowsKeys);
+                if (lane == 0) (is_v ? vmeta + st * 8 : kmeta + (j % kRowsMeta) * 8)[w] = m;
             }
             fence_proxy_async();
             __syncwarp();
@@ -458,10 +343,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 ok = __all_sync(0xffffffffu, ok);
                 __threadfence_block();
             };
-            // exponent of a place of a tile
-            auto exp_of = [&](const uint32_t *unit, const int8_t *place, uint32_t k) -> int {
-                return unit[k / 8] >> 24 ? (int)place[k] : meta_exp(unit[k / 8]);
-            };
             // O of the tile before into the sums: acc = acc * corr + O * osc
             auto take_o = [&]() {
                 const uint32_t col = tm_o + lanes + half * (HD / 2);
@@ -481,26 +362,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                         acc[c / 2 + k] = fma2(pair(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), o2, acc[c / 2 + k]);
                 }
             };
-            // places of the 32 from key0 that this row sees
-            auto visible = [&](uint32_t key0) -> uint32_t {
-                uint32_t vis = 0xFFFFFFFFu;
-                if (key0 + 32 > ctx) {
-                    if (a.tree != nullptr) {
-                        if (key0 >= ctx) {
-                            const uint32_t sh = key0 - ctx;
-                            vis = sh < 64 ? (uint32_t)(mask >> sh) : 0;
-                        } else {
-                            const uint32_t sh = ctx - key0;  // 1..31
-                            vis = (uint32_t)(mask << sh) | ((1u << sh) - 1);
-                        }
-                    } else {
-                        const uint32_t seen = ctx + tok + 1;  // places 0 .. seen - 1
-                        vis = seen >= key0 + 32 ? 0xFFFFFFFFu : seen <= key0 ? 0 : (1u << (seen - key0)) - 1;
-                    }
-                }
-                if (key0 + 32 > places) vis &= places <= key0 ? 0 : (1u << (places - key0)) - 1;
-                return vis;
-            };
+            auto visible = [&](uint32_t key0) { return rows_visible(a.tree != nullptr, mask, tok, ctx, places, key0); };
             // One tile. Units of K or V of different scale and marked places are rare and cost the
             // others nothing: they have a copy of the code of their own (in one, the branches and
             // what they keep in registers slowed every tile by 5 to 9 percent).
@@ -526,7 +388,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_empty);
                 sum16(16);
-                float cqk = cq * pow2i(meta_exp(km.x));
+                float cqk = score_factor(cq, meta_exp(km.x));
                 uint32_t vis = key0 + 32 > ctx ? visible(key0) : 0xFFFFFFFFu;
                 if (RARE && !meta_plain(km)) {
                     const uint32_t bad = meta_bytes(km, 0);
@@ -739,49 +601,61 @@ static int attn_rows_check(const b2_attn_rows_args *a)
     return 0;
 }
 
-// Kernel, blocks and splits. Up to kFewRows rows of an (item, KV head) go to
-// attn_few_kernel, which converts K and V in registers and multiplies with mma.sync: no
-// tensor-memory set-up, no roles to synchronise, no 128-row products for a handful of
-// rows (8B shape: 8 tokens at context 1000 15.3 us against 17.8, one token at context
-// 4096 22.7 against 26.0, 32 sequences of it 217 against 231; with 48 rows of head size
-// 64 it loses, 50 against 29).
+constexpr uint32_t kFewCtx = 2048;
+constexpr uint32_t kLaidBlocks = 4;
+constexpr size_t kLaidBytes = (size_t)512 << 20;
+
+// Kernel, blocks and splits. Up to kFewRows rows of an (item, KV head) over up to kFewCtx
+// places go to attn_few_kernel, which converts K and V in registers and multiplies with
+// mma.sync: no tensor-memory set-up, no roles to synchronise, no 128-row products for a
+// handful of rows, no second kernel. Against attn_rows_kernel, one token of the 8B shape
+// (4 rows) at context 1000 9.9 us and 15.1, 1900 13.4 and 18.1, 4000 22.9 and 23.0; 8
+// sequences of it 24.7 and 25.6, 39.6 and 39.0, 72.0 and 71.9. (For 32 rows it lost: 8
+// sequences of 8 tokens at context 1000 35 and 28.)
 //
-// The splits take the least modelled time, in quarters of a tile's: a CTA costs kSetup
-// besides its tiles (launch, q, the pipeline's ends), joining kJoin and one per split,
-// within a cluster half of kJoin. Measured (8B shape, attn_rows_kernel): context 1000
-// with 8 tokens 8 splits 17.8 us, 16 splits 21.2, 4 19.0; one KV head of the 70B shape,
-// 8 sequences of 30000 18 splits 82.8 us, 12 97.9, 24 98.2.
+// From kLaidBlocks blocks of 128 rows on, K and V are laid out as operands once for all of
+// them (b2_attn_laid.cu). 2000 cached places, laid out and each block for itself: 8B shape,
+// 8 sequences of 128 rows (4 blocks) 122 us and 138, 512 rows (16 blocks) 67 and 94; 8
+// sequences of 64 (2 blocks) 82 and 79.5; 9 heads of 64, 8 sequences of 64 rows (2 blocks)
+// 35.7 and 30.7. That takes scratch of the size of the batch's K and V, and is left out
+// where it would be more than kLaidBytes.
+//
+// The splits take the least modelled time, in quarters of a tile's: what a CTA costs besides
+// its tiles (launch, q, the pipeline's ends) and what joining costs, by a kernel also one
+// per split. Measured (8B shape, attn_rows_kernel): 8 tokens at context 1000 8 splits 17.8
+// us, 16 splits 21.2, 4 19.0; one KV head of the 70B shape, 8 sequences of 30000 18 splits
+// 82.8 us, 12 97.9, 24 98.2.
 static void attn_rows_plan(const b2_attn_rows_args *a, RowsParams &p, bool &few)
 {
     p.group = a->n_heads / a->n_kv_heads;
     const uint64_t rows = (uint64_t)a->max_rows * p.group, sms = (uint64_t)sm_count();
-    few = rows <= kFewRows;
-    p.block = !few ? kRowsM : rows <= 16 ? 16 : 32;
-    p.unit = few ? kFewUnit : kRowsKeys;
+    few = rows <= kFewRows && a->max_ctx <= kFewCtx;
+    p.block = few ? kFewRows : kRowsM;
     p.blocks = (uint32_t)((rows + p.block - 1) / p.block);
-    const uint64_t ctas = (uint64_t)a->batch * a->n_kv_heads * p.blocks;
-    // a tile: 64 places of a tcgen05 CTA, or a pass of 16 places per warp
-    const uint64_t tile = few ? kFewUnit * kFewWarps : kRowsKeys, tiles = (a->max_ctx + tile - 1) / tile;
-    constexpr uint64_t kSetup = 4 * 4, kJoin = 2 * 4;  // quarters of a tile
+    const uint64_t ctas = (uint64_t)a->batch * a->n_kv_heads * p.blocks, pairs = (a->max_ctx + kLaidKeys - 1) / kLaidKeys;
+    const bool laid = !few && p.blocks >= kLaidBlocks && (uint64_t)a->batch * a->n_kv_heads * pairs <= kLaidBytes / attn_laid_pair(a->head_dim);
+    p.pairs = laid ? (uint32_t)pairs : 0;
+    p.unit = few ? kFewUnit : laid ? kLaidKeys : kRowsKeys;
+    // a tile: 64 places of a tcgen05 CTA (128 laid out), or a pass of 16 places per warp
+    const uint64_t tile = few ? kFewUnit * kFewWarps : p.unit, tiles = (a->max_ctx + tile - 1) / tile;
+    const uint64_t setup = few ? 6 : 16, join = few ? 1 : 8;  // quarters of a tile
     uint64_t best = ~0ull;
     p.splits = 1;
-    for (uint64_t s = 1; s <= kRowsMaxSplits && s <= tiles; s = few ? 2 * s : s + 1) {
+    for (uint64_t s = 1; s <= (few ? kFewCluster : kRowsMaxSplits) && s <= tiles; s = few ? 2 * s : s + 1) {
         const uint64_t waves = (ctas * s + sms - 1) / sms;
-        // (the few kernel joins up to kFewCluster splits itself)
-        const uint64_t join = s == 1 ? 0 : few && s <= kFewCluster ? kJoin / 2 : kJoin + s;
-        const uint64_t cost = waves * (4 * ((tiles + s - 1) / s) + kSetup) + join;
+        const uint64_t cost = waves * (4 * ((tiles + s - 1) / s) + setup) + (s == 1 ? 0 : few ? join : join + s);
         if (cost < best) {
             best = cost;
             p.splits = (uint32_t)s;
         }
     }
-    p.cluster = few && p.splits > 1 && p.splits <= kFewCluster;
 }
 
-static size_t attn_rows_scratch(const b2_attn_rows_args *a, const RowsParams &p)
+static size_t attn_rows_scratch(const b2_attn_rows_args *a, const RowsParams &p, bool few)
 {
-    if (p.splits == 1 || p.cluster) return 0;
-    return (size_t)a->batch * a->n_kv_heads * p.blocks * p.splits * p.block * (a->head_dim + 4) * sizeof(float);
+    const size_t laid = (size_t)a->batch * a->n_kv_heads * p.pairs * attn_laid_pair(a->head_dim);
+    if (p.splits == 1 || few) return laid;
+    return laid + (size_t)a->batch * a->n_kv_heads * p.blocks * p.splits * p.block * (a->head_dim + 4) * sizeof(float);
 }
 
 static cudaError_t launch_rows_attn(const void *fn, dim3 grid, int threads, size_t smem, int pdl, cudaStream_t st, const RowsParams &p)
@@ -810,7 +684,7 @@ extern "C" size_t b2_attn_rows_scratch_bytes(const b2_attn_rows_args *a)
     RowsParams p = {};
     bool few;
     attn_rows_plan(a, p, few);
-    return attn_rows_scratch(a, p);
+    return attn_rows_scratch(a, p, few);
 }
 
 extern "C" int b2_attn_rows(const b2_attn_rows_args *a, void *stream)
@@ -822,13 +696,16 @@ extern "C" int b2_attn_rows(const b2_attn_rows_args *a, void *stream)
     bool few;
     attn_rows_plan(a, p, few);
     if ((uint64_t)a->n_kv_heads * p.blocks > 65535u) return -9;
-    const size_t need = attn_rows_scratch(a, p);
+    const size_t need = attn_rows_scratch(a, p, few);
     if (need > 0 && (a->scratch == nullptr || a->scratch_bytes < need || ((uintptr_t)a->scratch & 15))) return -1;
-    p.part = (float *)a->scratch;
+    p.laid = (uint8_t *)a->scratch;
+    p.part = (float *)((uint8_t *)a->scratch + (size_t)a->batch * a->n_kv_heads * p.pairs * attn_laid_pair(a->head_dim));
     p.scale = (float)(1.4426950408889634 / sqrt((double)a->head_dim));
     const cudaStream_t st = (cudaStream_t)stream;
     if (few) {
         if (attn_few_launch(p, st) != cudaSuccess) return -8;
+    } else if (p.pairs != 0) {
+        if (attn_laid_launch(p, st) != cudaSuccess) return -8;
     } else {
         const bool wide = a->head_dim > 64;
         const void *fn = a->head_dim == 128  ? (const void *)attn_rows_kernel<128, true>
@@ -840,7 +717,7 @@ extern "C" int b2_attn_rows(const b2_attn_rows_args *a, void *stream)
         if (launch_rows_attn(fn, dim3(p.splits, a->n_kv_heads * p.blocks, a->batch), kRowsThreads, smem, a->pdl, st, p) != cudaSuccess)
             return -8;
     }
-    if (p.splits > 1 && !p.cluster) {
+    if (p.splits > 1 && !few) {
         const uint32_t rows = a->max_rows * p.group;
         if (launch_rows_attn((const void *)attn_rows_join_kernel, dim3((rows + kJoinWarps - 1) / kJoinWarps, a->n_kv_heads, a->batch),
                              kJoinWarps * 32, 0, a->pdl, st, p) != cudaSuccess)

@@ -29,6 +29,15 @@ __host__ __device__ constexpr uint32_t umma_idesc_bf16(uint32_t m, uint32_t n)
     return umma_idesc_f16(m, n) | (1u << 7) | (1u << 10);
 }
 
+// True in one thread of a full warp, always the same one. (Under it the compiler keeps
+// the descriptors of MMAs in uniform registers, which it does not under a lane's number.)
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // One kind::f16 MMA (the operand type is the instruction descriptor's).
 __device__ __forceinline__ void umma_16(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {

@@ -376,6 +376,131 @@ def test_attn_pool_past_32_bits(b2, torch):
     assert np.abs(got - s.reference()).max() <= ATTN_TOL * 5
 
 
+@pytest.mark.parametrize("new", [15, 16, 17, 127, 128, 129, 384, 385])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attn_row_counts(b2, torch, hd, new):
+    """Around the numbers of rows at which another kernel or block starts."""
+    Scene(torch, 1, 1, hd, 64, [300], [new], tree=new <= 64, seed=new).check(b2)
+
+
+@pytest.mark.parametrize("ctx", [2046, 2047, 2048])
+def test_attn_one_token_at_long_contexts(b2, torch, ctx):
+    Scene(torch, 4, 1, 64, 64, [ctx, 1, 17, 0, 1000], [1, 1, 1, 1, 1], seed=ctx).check(b2)
+    Scene(torch, 4, 4, 128, 64, [ctx, 130], [2, 1], seed=ctx).check(b2)
+
+
+@pytest.mark.parametrize("h,hkv,hd", [(16, 2, 128), (8, 1, 64), (16, 2, 80), (10, 1, 32)])
+@pytest.mark.parametrize("ctx", [[0], [1], [64, 127], [128, 0, 500], [2500]])
+def test_attn_many_rows_of_trees(b2, torch, h, hkv, hd, ctx):
+    """Four blocks of 128 rows and more share an item's K and V."""
+    Scene(torch, h, hkv, hd, 16, ctx, [64] + [41, 0, 9][:len(ctx) - 1], seed=h + hd).check(b2)
+
+
+def test_attn_many_rows_of_ragged_chunks(b2, torch):
+    Scene(torch, 8, 2, 128, 24, [500, 40, 0, 1, 63], [400, 0, 129, 1, 65], tree=False, seed=30, q_pad=4).check(b2)
+    Scene(torch, 4, 1, 64, 64, [3000], [130], tree=False, seed=31).check(b2)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, 3e38, 1e10])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("victim", [3, 40])
+def test_attn_many_rows_masked_places(b2, torch, which, bad, victim):
+    s = Scene(torch, 8, 1, 128, 16, [90], [64], seed=32)
+    ref = s.reference()
+    pg, off = s.place(0, 90 + victim)
+    getattr(s, which)[pg, :, off] = bad
+    got, err = s.run(b2)
+    hits = 0
+    for i in range(64):
+        if s.masks[i] >> victim & 1:
+            hits += 1
+            if not np.isfinite(bad):
+                assert np.isnan(got[i]).all()
+        else:
+            assert np.abs(got[i] - ref[i]).max() <= ATTN_TOL * 5
+    assert hits > 0 and (np.isfinite(bad) or err == ERR_NONFINITE)
+
+
+def test_attn_many_rows_of_mixed_sizes(b2, torch):
+    s = Scene(torch, 8, 1, 128, 16, [300], [64], seed=33)
+    s.v *= np.ldexp(np.float32(1), np.random.default_rng(8).integers(-14, 15, s.v.shape[0] * 16)).reshape(-1, 1, 16, 1).astype(np.float32)
+    got, err = s.run(b2)
+    assert err == 0
+    ref, s.v = s.reference(), np.abs(s.v)
+    assert (np.abs(got - ref) <= ATTN_TOL * s.reference().max(-1, keepdims=True) + 2.0 ** -24).all()
+
+
+def test_attn_many_rows_refused_items_and_pages(b2, torch):
+    s = Scene(torch, 8, 1, 64, 16, [200, 30], [64, 5], seed=34)
+    s.table[0, 2] = -1
+    s.q[s.start[1] + 1, 3] = np.nan
+    got, err = s.run(b2)
+    assert err == ERR_POSITION | ERR_NONFINITE
+    keep = s.sees
+    s.sees = lambda b, i: [j for j in keep(b, i) if b or j // 16 != 2]
+    s.table[0, 2] = 0
+    s.k, s.v, s.q = np.nan_to_num(s.k), np.nan_to_num(s.v), np.nan_to_num(s.q)
+    ref = s.reference()
+    assert np.isnan(got[s.start[1] + 1, 0]).all()
+    got[s.start[1] + 1, 0] = ref[s.start[1] + 1, 0]
+    assert np.abs(got - ref).max() <= ATTN_TOL * 5
+    s.ctx = np.array([200, 900])
+    got, err = s.run(b2, max_ctx=264)
+    assert err == ERR_POSITION and (got[64:] == 7.25).all()
+
+
+def test_attn_many_rows_without_room_for_operands(b2, torch):
+    """A bound on the places so large that K and V are not laid out in scratch gives the same within both bounds."""
+    s = Scene(torch, 8, 1, 128, 64, [150], [64], seed=35)
+    ref = s.reference()
+    a = s.args(b2)
+    small = a.scratch_bytes
+    s.pps = 9000
+    wide = np.full((1, s.pps), -7, np.int32)
+    wide[:, :s.table.shape[1]] = s.table
+    s.table = wide
+    a = s.args(b2, max_ctx=64 * 9000)
+    assert 0 < small < 1 << 20 and a.scratch_bytes < 512 << 20
+    assert b2.lib().b2_attn_rows(a, None) == 0
+    torch.cuda.synchronize()
+    got = s.d["out"].cpu().numpy()[:s.rows, :8 * 128].reshape(s.rows, 8, 128)
+    assert int(s.d["err"].item()) == 0 and np.abs(got - ref).max() <= ATTN_TOL * 5
+
+
+def test_attn_many_rows_graph_and_streams(b2, torch):
+    """Captured and replayed with other lengths; calls at once with scratch of their own; the same bits each time."""
+    s = Scene(torch, 8, 1, 128, 64, [900, 30], [64, 50], seed=36)
+    t = Scene(torch, 8, 1, 64, 64, [300, 500], [60, 64], seed=37)
+    a, b = s.args(b2), t.args(b2)
+    st, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    b2.check("warm", b2.lib().b2_attn_rows(a, st.cuda_stream))
+    st.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        b2.check("capture", b2.lib().b2_attn_rows(a, torch.cuda.current_stream().cuda_stream))
+    first = None
+    for ctx in ([900, 30], [100, 11], [900, 30]):
+        s.ctx = np.array(ctx)
+        s.k, s.v = np.nan_to_num(s.k), np.nan_to_num(s.v)
+        s.table = np.abs(s.table) % s.pool_pages
+        for name, x in (("k", s.k), ("v", s.v), ("table", s.table), ("ctx", s.ctx.astype(np.int32))):
+            s.d[name].copy_(dev(torch, x))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            with torch.cuda.stream(st):
+                g.replay()
+            b2.check("beside", b2.lib().b2_attn_rows(b, s2.cuda_stream))
+        torch.cuda.synchronize()
+        got = s.d["out"].cpu().numpy()[:s.rows, :8 * 128].reshape(s.rows, 8, 128)
+        assert np.abs(got - s.reference()).max() <= ATTN_TOL * 5
+        if ctx == [900, 30]:
+            assert first is None or (got == first).all()
+            first = got
+    got = t.d["out"].cpu().numpy()[:t.rows, :8 * 64].reshape(t.rows, 8, 64)
+    assert np.abs(got - t.reference()).max() <= ATTN_TOL * 5
+
+
 def test_attn_matches_single_query_attention(b2, torch):
     """One row per item is b2_attn's case: the same numbers within both bounds."""
     s = Scene(torch, 8, 2, 128, 64, [300, 77, 0], [1, 1, 1], seed=20)
