@@ -500,8 +500,11 @@ int b2_rows_append(const b2_rows_append_args *a, void *stream);
  * whose lengths do not fit (max_rows, rows, max_ctx, B2_MAX_TREE) or a
  * negative page id (or, with pool_pages given, one past the pool) raises
  * B2_ERR_POSITION; such an item's rows are left as they were, such a page's
- * places are not seen. Products are kept to about 2^-22 (see the kernel); the
- * result does not depend on timing. */
+ * places are not seen. Products are of 22-bit operands, absolutely no finer than
+ * 2^-25 where the largest of neighbouring places is between 2^-4 and 2^12, and
+ * relative to it outside; a place far above its neighbours takes nothing from
+ * them. The result does not depend on timing. Scratch grows with batch, rows and
+ * max_ctx (many rows per item: up to 512 MB for K and V laid out as operands). */
 typedef struct b2_attn_rows_args {
     uint32_t batch, n_heads, n_kv_heads, head_dim; /* head_dim a multiple of 16, at most 128 */
     uint32_t max_rows;           /* most rows of one item (sizes the grid) */
