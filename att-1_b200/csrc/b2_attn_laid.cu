@@ -194,20 +194,28 @@ __global__ void __launch_bounds__(kLaidThreads, 1) attn_laid_kernel(const RowsPa
              *o_empty = o_full + 2, *q_full = o_empty + 1, *done = q_full + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 2);
 
-    pdl_wait();
+    // Launched while attn_rows_lay_kernel still runs: what came before that has completed, and
+    // only the copies read what it writes.
     pdl_launch_dependents();
     uint32_t r0, n, ctx;
     if (!rows_item(a, item, r0, n, ctx)) {
         if (threadIdx.x == 0 && split == 0 && blockIdx.y == 0) raise_error(a.err, B2_ERR_POSITION);
+        pdl_wait();
         return;
     }
     const uint32_t mrows = n * p.group;  // rows of this (item, KV head)
-    if (blk * kRowsM >= mrows) return;
+    if (blk * kRowsM >= mrows) {
+        pdl_wait();
+        return;
+    }
     const uint32_t live = min(kRowsM, mrows - blk * kRowsM);
     const uint32_t places = rows_places(p, n, ctx, blk);
     uint32_t t0, t1;
     rows_range(p, places, split, t0, t1);
-    if (t0 == t1) return;  // the joining kernel skips the same splits
+    if (t0 == t1) {  // the joining kernel skips the same splits
+        pdl_wait();
+        return;
+    }
     const uint32_t np = t1 - t0, nt = 2 * np;  // pairs of tiles, tiles
     const uint32_t nq = (live + 31) / 32;  // quarters of the rows in use
 
@@ -247,6 +255,7 @@ __global__ void __launch_bounds__(kLaidThreads, 1) attn_laid_kernel(const RowsPa
                 const uint8_t *src = p.laid + (((size_t)item * a.n_kv_heads + kvh) * p.pairs + t0) * P::bytes;
                 bool ok = true;
                 uint32_t i = 0;
+                pdl_wait();
                 // (no copy is in flight when the CTA ends, not even after a wait that gave up)
                 if (warp == kLaidCopyWarp) {
                     for (; i < np; ++i, src += P::bytes) {
@@ -532,7 +541,7 @@ template <int HD, bool EXACT>
 static cudaError_t launch_laid(const RowsParams &p, cudaStream_t st)
 {
     const b2_attn_rows_args &a = p.a;
-    auto launch = [&](void (*kernel)(const RowsParams), dim3 grid, uint32_t threads, uint32_t smem) {
+    auto launch = [&](void (*kernel)(const RowsParams), dim3 grid, uint32_t threads, uint32_t smem, int pdl) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
         cudaLaunchConfig_t cfg = {};
@@ -542,13 +551,13 @@ static cudaError_t launch_laid(const RowsParams &p, cudaStream_t st)
         cfg.stream = st;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = a.pdl ? 1 : 0;
+        attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         return cudaLaunchKernelEx(&cfg, kernel, p);
     };
-    const cudaError_t e = launch(attn_rows_lay_kernel<HD, EXACT>, dim3(2 * p.pairs, a.n_kv_heads, a.batch), kLayWarps * 32, kRowsKeys * 2 * HD * 4);
-    return e != cudaSuccess ? e : launch(attn_laid_kernel<HD>, dim3(p.splits, a.n_kv_heads * p.blocks, a.batch), kLaidThreads, LaidSmem<HD>::bytes);
+    const cudaError_t e = launch(attn_rows_lay_kernel<HD, EXACT>, dim3(2 * p.pairs, a.n_kv_heads, a.batch), kLayWarps * 32, kRowsKeys * 2 * HD * 4, a.pdl);
+    return e != cudaSuccess ? e : launch(attn_laid_kernel<HD>, dim3(p.splits, a.n_kv_heads * p.blocks, a.batch), kLaidThreads, LaidSmem<HD>::bytes, 1);
 }
 
 size_t attn_laid_pair(uint32_t head_dim) { return head_dim > 64 ? LaidPair<128>::bytes : LaidPair<64>::bytes; }

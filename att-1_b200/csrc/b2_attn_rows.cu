@@ -717,10 +717,10 @@ extern "C" int b2_attn_rows(const b2_attn_rows_args *a, void *stream)
         if (launch_rows_attn(fn, dim3(p.splits, a->n_kv_heads * p.blocks, a->batch), kRowsThreads, smem, a->pdl, st, p) != cudaSuccess)
             return -8;
     }
-    if (p.splits > 1 && !few) {
+    if (p.splits > 1 && !few) {  // (launched early in any case: it waits for the kernel before)
         const uint32_t rows = a->max_rows * p.group;
         if (launch_rows_attn((const void *)attn_rows_join_kernel, dim3((rows + kJoinWarps - 1) / kJoinWarps, a->n_kv_heads, a->batch),
-                             kJoinWarps * 32, 0, a->pdl, st, p) != cudaSuccess)
+                             kJoinWarps * 32, 0, 1, st, p) != cudaSuccess)
             return -8;
     }
     return 0;

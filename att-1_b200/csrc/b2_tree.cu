@@ -47,7 +47,7 @@ __device__ __forceinline__ uint32_t plan_find(const uint32_t *start, uint32_t n,
 // Every CTA forms the exclusive prefix sums of the new rows and of the fresh
 // pages over all sequences in shared memory (16 bytes per sequence; reading the
 // three length arrays from L2 costs each CTA about a microsecond, less than a
-// second launch or a wait between CTAs would), judges the step as a whole, and
+// second launch or a wait between CTAs would), checks the step as a whole, and
 // then writes its share of the rows and of the fresh pages. A row's page is
 // read from the table below mapped[b] and computed from the free stack above,
 // so no CTA depends on another's table writes.
