@@ -684,7 +684,7 @@ extern "C" size_t b2_attn_rows_scratch_bytes(const b2_attn_rows_args *a)
     RowsParams p = {};
     bool few;
     attn_rows_plan(a, p, few);
-    return attn_rows_scratch(a, p, few);
+    return (uint64_t)a->n_kv_heads * p.blocks > 65535u ? 0 : attn_rows_scratch(a, p, few);
 }
 
 extern "C" int b2_attn_rows(const b2_attn_rows_args *a, void *stream)

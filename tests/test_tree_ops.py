@@ -926,6 +926,70 @@ def test_compact_bad_rows(b2, torch):
 # ---- the operators together ----------------------------------------------------------------------------
 
 
+@pytest.mark.parametrize("h,hkv,hd", [(8, 1, 64), (4, 2, 128), (2, 2, 48)])
+def test_steps_of_chunks(b2, torch, h, hkv, hd):
+    """Three steps of prompt chunks over several layers that share one scratch, each kernel launched while
+    the one before still runs: every row against float64."""
+    batch, page, layers, pps = 3, 16, 5, 40
+    rng = np.random.default_rng(hd)
+    L = b2.lib()
+    pool = batch * pps
+    free = dev(torch, rng.permutation(pool), np.int32)
+    ctx = torch.zeros(batch, dtype=torch.int32, device="cuda")
+    mapped, count = torch.zeros_like(ctx), dev(torch, [pool], np.int32)
+    table = torch.full((batch, pps), -1, dtype=torch.int32, device="cuda")
+    k, v = (torch.full((layers, pool, hkv, page, hd), float("nan"), device="cuda") for _ in range(2))
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    K, V = ([[np.zeros((0, hkv, hd))] * batch for _ in range(layers)] for _ in range(2))
+    scratch = None
+    for new in ([200, 0, 130], [1, 70, 260], [64, 3, 1]):
+        rows, start = sum(new), np.concatenate([[0], np.cumsum(new)])
+        nd = dev(torch, new, np.int32)
+        d = {x: torch.full((rows,), -1, dtype=torch.int32, device="cuda") for x in ("item", "pos", "slot")}
+        rs = torch.zeros(batch + 1, dtype=torch.int32, device="cuda")
+        mo, fo = torch.zeros_like(mapped), torch.zeros_like(count)
+        ys = rng.normal(0, 1, (layers, rows, (h + 2 * hkv) * hd)).astype(np.float32)
+        y = dev(torch, ys)
+        q, o = (torch.zeros(layers, rows, h * hd, device="cuda") for _ in range(2))
+        kvs = [b2.KVLayout(p(k[l]), p(v[l]), p(table), page, pps, hkv, hd) for l in range(layers)]
+        calls = [b2.AttnRowsArgs(batch=batch, n_heads=h, n_kv_heads=hkv, head_dim=hd, max_rows=max(new), rows=rows, q=p(q[l]),
+                                 q_stride=h * hd, kv=kvs[l], pool_pages=pool, row_start=p(rs), ctx_len=p(ctx), max_ctx=pps * page,
+                                 ctx=p(o[l]), ctx_stride=h * hd, err=p(err), pdl=1) for l in range(layers)]
+        need = L.b2_attn_rows_scratch_bytes(calls[0])
+        if scratch is None or scratch.numel() < need:
+            scratch = torch.empty(need + 16, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        b2.check("plan", L.b2_kv_plan(b2.KvPlanArgs(
+            batch=batch, max_rows=rows, page_tokens=page, pages_per_seq=pps, pool_pages=pool, ctx_len=p(ctx), new_len=p(nd),
+            mapped=p(mapped), free_pages=p(free), free_count=p(count), page_table=p(table), mapped_out=p(mo), free_out=p(fo),
+            row_start=p(rs), row_item=p(d["item"]), row_pos=p(d["pos"]), row_slot=p(d["slot"]), err=p(err), pdl=1), None))
+        for l, a in enumerate(calls):
+            b2.check("append", L.b2_rows_append(b2.RowsAppendArgs(
+                m=rows, y=p(y[l]), y_stride=y.shape[2], q_rows=h * hd, q=p(q[l]), q_stride=h * hd, slots=p(d["slot"]), kv=kvs[l],
+                pool_pages=pool, err=p(err), pdl=1), None))
+            a.scratch, a.scratch_bytes = p(scratch), scratch.numel()
+            b2.check("attn", L.b2_attn_rows(a, None))
+        torch.cuda.synchronize()
+        assert int(err.item()) == 0
+        got = o.cpu().numpy().reshape(layers, rows, hkv, h // hkv, hd)
+        yy = ys.astype(np.float64).reshape(layers, rows, h + 2 * hkv, hd)
+        for l in range(layers):
+            for b in range(batch):
+                at = slice(start[b], start[b + 1])
+                K[l][b] = np.concatenate([K[l][b], yy[l, at, h:h + hkv]])
+                V[l][b] = np.concatenate([V[l][b], yy[l, at, h + hkv:]])
+                if new[b] == 0:
+                    continue
+                t = len(K[l][b])
+                s = np.einsum("nhgd,thd->nhgt", yy[l, at, :h].reshape(-1, hkv, h // hkv, hd), K[l][b]) / np.sqrt(hd)
+                s = np.where((np.arange(t) <= t - new[b] + np.arange(new[b])[:, None])[:, None, None], s, -np.inf)
+                w = np.exp(s - s.max(-1, keepdims=True))
+                want = np.einsum("nhgt,thd->nhgd", w / w.sum(-1, keepdims=True), V[l][b])
+                assert np.abs(got[l, at] - want).max() <= ATTN_TOL * 5
+        ctx += nd
+        mapped, count = mo, fo
+
+
 def test_step_of_trees(b2, torch):
     """Two steps of ragged trees: plan, append, attention, verification and compaction; afterwards the
     cache holds what a plain replay of the taken tokens holds, and attention over it agrees."""
