@@ -31,10 +31,10 @@
 // hi hi + lo hi + hi lo with f32 accumulation; what is dropped is below 2^-22.
 // f16 rather than bf16 pairs (2^-16) because the scale takes care of the range:
 // a row of q, eight places' K and eight places' V have a power of two each, 1 for
-// largest magnitudes from 1 to 2^12, else what brings the largest to [1, 16). So an
-// element down to 2^-9 (of the largest, where that was scaled) still keeps 16 bits,
-// and what a smaller one loses is below 2^-25. (The scaling exponents are multiples
-// of four, so that neighbours mostly share one, and mostly have none to apply.) A
+// largest magnitudes from 2^-4 to 2^12, else what brings the largest to [1, 16). So an
+// element keeps 22 bits down to 2^-3, and what a smaller one loses is below 2^-25 (both
+// of 1, or of the scaled largest). The scaling exponents are multiples of four, so that
+// neighbours mostly share one, and mostly have none to apply. A
 // place of 2^12 and more that is far above one of its neighbours gets its own scale,
 // as they do: a place that a row does not see, or gives no weight, takes nothing from
 // the others, whatever it holds. K's scale goes into the scores; V's into P, relative
