@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(kCompactThreads)
     kv_compact_kernel(const CompactLayers L, b2_kv_layout kv, uint32_t pool_pages, const int32_t *ctx_len,
                       const int32_t *path, const int32_t *count, int32_t *err)
 {
-    __shared__ uint32_t src[B2_MAX_TREE], dst[B2_MAX_TREE];  // (page, offset in page), packed as pool places
+    __shared__ uint2 src[B2_MAX_TREE], dst[B2_MAX_TREE];  // page, offset in page
     __shared__ uint32_t moves;
     pdl_wait();
     pdl_launch_dependents();
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kCompactThreads)
         for (uint32_t i0 = 0; i0 < B2_MAX_TREE; i0 += 32) {
             const uint32_t i = i0 + lane;
             bool move = false;
-            uint32_t s = 0, d = 0;
+            uint2 s = make_uint2(0, 0), d = s;
             if (fault == 0 && i < (uint32_t)n) {
                 const int32_t p = path[(size_t)item * B2_MAX_TREE + i];
                 if (p < (int32_t)i || p >= B2_MAX_TREE || (uint32_t)c + (uint32_t)p >= cap) {
@@ -362,8 +362,8 @@ __global__ void __launch_bounds__(kCompactThreads)
                     const int32_t ps = row[at / kv.page_tokens], pd = row[to / kv.page_tokens];
                     move = ps >= 0 && pd >= 0 && (pool_pages == 0 || ((uint32_t)ps < pool_pages && (uint32_t)pd < pool_pages));
                     if (!move) fault = B2_ERR_POSITION;
-                    s = (uint32_t)ps * kv.page_tokens + at % kv.page_tokens;
-                    d = (uint32_t)pd * kv.page_tokens + to % kv.page_tokens;
+                    s = make_uint2((uint32_t)ps, at % kv.page_tokens);
+                    d = make_uint2((uint32_t)pd, to % kv.page_tokens);
                 }
             }
             const uint32_t who = __ballot_sync(0xffffffffu, move);
@@ -387,15 +387,15 @@ __global__ void __launch_bounds__(kCompactThreads)
 #pragma unroll
             for (uint32_t j = 0; j < kCompactBatch; ++j) {
                 if (i0 + j < n) {
-                    const uint32_t s = src[i0 + j];
-                    x[j] = pool[(((size_t)(s / kv.page_tokens) * kv.n_kv_heads + head) * kv.page_tokens + s % kv.page_tokens) * cols];
+                    const uint2 s = src[i0 + j];
+                    x[j] = pool[(((size_t)s.x * kv.n_kv_heads + head) * kv.page_tokens + s.y) * cols];
                 }
             }
 #pragma unroll
             for (uint32_t j = 0; j < kCompactBatch; ++j) {
                 if (i0 + j < n) {
-                    const uint32_t d = dst[i0 + j];
-                    pool[(((size_t)(d / kv.page_tokens) * kv.n_kv_heads + head) * kv.page_tokens + d % kv.page_tokens) * cols] = x[j];
+                    const uint2 d = dst[i0 + j];
+                    pool[(((size_t)d.x * kv.n_kv_heads + head) * kv.page_tokens + d.y) * cols] = x[j];
                 }
             }
         }
@@ -499,9 +499,7 @@ extern "C" int b2_kv_compact(const b2_kv_compact_args *a, void *stream)
             k.pages_per_seq != kv.pages_per_seq || k.n_kv_heads != kv.n_kv_heads || k.head_dim != kv.head_dim)
             return -1;
     }
-    if ((uint64_t)kv.pages_per_seq * kv.page_tokens > 0x7FFFFFFFull ||
-        (uint64_t)a->pool_pages * kv.page_tokens > 0xFFFFFFFFull)
-        return -1;
+    if ((uint64_t)kv.pages_per_seq * kv.page_tokens > 0x7FFFFFFFull) return -1;
     const uint32_t work = 2 * kv.n_kv_heads * (kv.head_dim / 4);
     uint32_t pool_pages = a->pool_pages;
     const int32_t *ctx_len = a->ctx_len, *path = a->path, *count = a->count;

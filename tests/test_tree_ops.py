@@ -911,6 +911,30 @@ def test_compact(b2, torch, layers, hkv, hd, page):
     assert err == 0 and (got == want).all()
 
 
+def test_compact_pool_past_32_bits_of_places(b2, torch):
+    """A pool of more than 2^32 places (69 GB of 16-byte rows; K and V the same)."""
+    page, n = 1 << 16, (1 << 16) + 3
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("not enough device memory free")
+    pool = torch.empty(n, page, 4, device="cuda")
+    table = dev(torch, [[n - 1, 2]], np.int32)
+    rows = torch.arange(40, dtype=torch.float32, device="cuda").reshape(10, 4) + 1
+    ctx = page - 3   # places page - 3 .. page + 6
+    pool[n - 1, page - 3:] = rows[:3]
+    pool[2, :7] = rows[3:]
+    pool[2, page - 10:] = 0
+    path = torch.full((1, 64), -1, dtype=torch.int32, device="cuda")
+    path[0, :4] = dev(torch, [0, 2, 5, 9], np.int32)
+    kv = (b2.KVLayout * 1)(b2.KVLayout(p(pool), p(pool), p(table), page, 2, 1, 4))
+    d = dict(ctx=dev(torch, [ctx], np.int32), count=dev(torch, [4], np.int32), err=torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert b2.lib().b2_kv_compact(b2.KvCompactArgs(n_layers=1, layers=kv, pool_pages=n, batch=1, ctx_len=p(d["ctx"]), path=p(path),
+                                                   count=p(d["count"]), err=p(d["err"])), None) == 0
+    torch.cuda.synchronize()
+    assert int(d["err"].item()) == 0
+    assert (pool[n - 1, page - 3:] == rows[[0, 2, 5]]).all()
+    assert (pool[2, 0] == rows[9]).all() and (pool[2, 1:7] == rows[4:]).all()
+
+
 def test_compact_bad_rows(b2, torch):
     got, want, err = compact_run(b2, torch, 2, 2, 64, 16, [10], [[0, 0, 5]])          # path below its index
     assert err == ERR_POSITION and (got == want).all()
