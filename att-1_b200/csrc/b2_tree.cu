@@ -241,15 +241,17 @@ __global__ void __launch_bounds__(2 * kAppendThreads) rows_append_kernel(const b
 
 constexpr int kAcceptWarps = 4;
 
-// One warp per item, rows i = lane and lane + 32. A row fits when its token is
-// the argmax token of its parent (the highest bit of its mask below itself)
-// and no earlier sibling carries the same token; with M the 64-bit set of
+// One warp per item, rows i = lane and lane + 32. A row's parent is the highest
+// bit of its mask below itself, and a tree's mask is its parent's and its own
+// bit, down to the root's. A row fits when its token is the argmax token of its
+// parent and no earlier sibling carries the same token; with M the 64-bit set of
 // fitting rows, a row is taken when its mask lies inside M. The taken rows are
 // one branch: two taken children of a row would carry the same token. All in
-// registers and one shared array; the time is two dependent load round trips.
+// registers and shared memory; the time is two dependent load round trips.
 __global__ void __launch_bounds__(kAcceptWarps * 32) tree_accept_kernel(const b2_tree_accept_args a)
 {
     __shared__ uint32_t tok_s[kAcceptWarps][64], next_s[kAcceptWarps][64];
+    __shared__ uint64_t mask_s[kAcceptWarps][64];
     __shared__ int8_t par_s[kAcceptWarps][64];
     pdl_wait();
     pdl_launch_dependents();
@@ -271,13 +273,22 @@ __global__ void __launch_bounds__(kAcceptWarps * 32) tree_accept_kernel(const b2
         const uint32_t i = lane + 32 * h;
         if (i < n) {
             mask[h] = a.tree != nullptr ? a.tree[r0 + i] : (2ull << i) - 1;
-            // itself, row 0, nothing after itself
-            tree[h] = (mask[h] >> i) == 1 && (mask[h] & 1);
-            if (!tree[h]) fault |= B2_ERR_TREE;
-            const uint64_t above = mask[h] & ((1ull << i) - 1);
-            par[h] = tree[h] && above != 0 ? 63 - __clzll(above) : -1;
+            mask_s[warp][i] = mask[h];
             tok[i] = a.tokens[r0 + i];
             nxt[i] = 0xFFFFFFFFu - (uint32_t)a.argmax[r0 + i];
+        }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t i = lane + 32 * h;
+        if (i < n) {
+            const uint64_t above = mask[h] & ((1ull << i) - 1);
+            const int up = 63 - __clzll(above);  // -1: none
+            // itself, nothing after itself, and all that its parent has
+            tree[h] = (mask[h] >> i) == 1 && (i == 0 || (up >= 0 && mask_s[warp][up] == above));
+            if (!tree[h]) fault |= B2_ERR_TREE;
+            par[h] = tree[h] ? up : -1;
             pr[i] = (int8_t)par[h];
         }
     }

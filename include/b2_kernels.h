@@ -532,9 +532,11 @@ int b2_attn_rows(const b2_attn_rows_args *a, void *stream);
  * no child does. path[b] = the local rows taken (ascending, row 0 first, -1
  * behind the last), count[b] how many, next[b] the last one's argmax token,
  * ctx_out[b] = ctx_len[b] + count[b]. An item without rows: count 0, next
- * 0xFFFFFFFF. A mask that no tree has (without its own bit or row 0, bits at or
- * past the row) raises B2_ERR_TREE and its row is not taken; a row count that
- * does not fit raises B2_ERR_POSITION (count 0). tree NULL: a chain. */
+ * 0xFFFFFFFF. A mask that no tree has (without its own bit, with bits past the
+ * row, or other than its parent's mask and its own bit, the parent being the
+ * last row before it that it names; the root names only itself) raises
+ * B2_ERR_TREE and neither its row nor those below it are taken; a row count
+ * that does not fit raises B2_ERR_POSITION (count 0). tree NULL: a chain. */
 typedef struct b2_tree_accept_args {
     uint32_t batch;
     uint32_t max_rows;           /* most rows of one item, at most B2_MAX_TREE */
