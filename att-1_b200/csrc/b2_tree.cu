@@ -365,8 +365,8 @@ __global__ void __launch_bounds__(kCompactThreads)
             bool move = false;
             uint2 s = make_uint2(0, 0), d = s;
             if (fault == 0 && i < (uint32_t)n) {
-                const int32_t p = path[(size_t)item * B2_MAX_TREE + i];
-                if (p < (int32_t)i || p >= B2_MAX_TREE || (uint32_t)c + (uint32_t)p >= cap) {
+                const int32_t *at_i = path + (size_t)item * B2_MAX_TREE + i, p = *at_i, before = i > 0 ? at_i[-1] : -1;
+                if (p < (int32_t)i || p <= before || p >= B2_MAX_TREE || (uint32_t)c + (uint32_t)p >= cap) {
                     fault = B2_ERR_POSITION;
                 } else if (p > (int32_t)i) {
                     const uint32_t at = (uint32_t)c + (uint32_t)p, to = (uint32_t)c + i;

@@ -556,9 +556,11 @@ typedef struct b2_tree_accept_args {
 int b2_tree_accept(const b2_tree_accept_args *a, void *stream);
 
 /* The K/V of the taken rows moved together in every layer: cache place
- * ctx_len[b] + path[b][i] to ctx_len[b] + i for i < count[b] (path[b][i] >= i,
- * ascending; others, and places outside the table row, raise B2_ERR_POSITION
- * and are not moved). ctx_len is the length before the step. */
+ * ctx_len[b] + path[b][i] to ctx_len[b] + i for i < count[b]. An entry below its
+ * index or not above the entry before it, and places outside the table row or on
+ * a bad page, raise B2_ERR_POSITION and are not moved; a count outside
+ * 0..B2_MAX_TREE or a negative ctx_len does so for the whole item. ctx_len is
+ * the length before the step. */
 typedef struct b2_kv_compact_args {
     uint32_t n_layers;
     const b2_kv_layout *layers;  /* host [n_layers], one geometry */

@@ -63,3 +63,13 @@ def test_accept_stops_before_a_mask_that_is_not_its_parents(b2, torch):
     r = accept_run(b2, torch, [0, 64], list(range(64)), masks, list(range(1, 65)), [0])
     # row 41's mask is no longer its parent's and its own bit either
     assert r["err"][0] == ERR_TREE and r["count"][0] == 40 and r["next"][0] == 40
+
+
+@pytest.mark.parametrize("path,moved", [([0, 5, 3], [0, 5]), ([0, 5, 5], [0, 5]), ([4, 3, 9], [4, None, 9]), ([0, -1, 7], [0, None, 7])])
+def test_compact_paths_that_do_not_ascend(b2, torch, path, moved):
+    got, want, err = compact_run(b2, torch, 2, 2, 64, 16, [10], [path], mutate=None)
+    assert err == ERR_POSITION
+    # the same call without the refused entries: each is left out by naming its own place
+    kept = [i if j is None else j for i, j in enumerate(moved)]
+    same, want, _ = compact_run(b2, torch, 2, 2, 64, 16, [10], [kept])
+    assert (same == want).all() and (got == want).all()
