@@ -358,13 +358,14 @@ __global__ void __launch_bounds__(kCompactThreads)
         const int32_t n = count[item], c = ctx_len[item];
         const uint32_t cap = kv.pages_per_seq * kv.page_tokens;
         const int32_t *row = L.table[layer] + (size_t)item * kv.pages_per_seq;
-        int fault = n < 0 || n > B2_MAX_TREE || c < 0 ? B2_ERR_POSITION : 0;
+        const bool fits = n >= 0 && n <= B2_MAX_TREE && c >= 0;
+        int fault = fits ? 0 : B2_ERR_POSITION;
         uint32_t kept = 0;
         for (uint32_t i0 = 0; i0 < B2_MAX_TREE; i0 += 32) {
             const uint32_t i = i0 + lane;
             bool move = false;
             uint2 s = make_uint2(0, 0), d = s;
-            if (fault == 0 && i < (uint32_t)n) {
+            if (fits && i < (uint32_t)n) {
                 const int32_t *at_i = path + (size_t)item * B2_MAX_TREE + i, p = *at_i, before = i > 0 ? at_i[-1] : -1;
                 if (p < (int32_t)i || p <= before || p >= B2_MAX_TREE || (uint32_t)c + (uint32_t)p >= cap) {
                     fault = B2_ERR_POSITION;

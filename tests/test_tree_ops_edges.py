@@ -73,3 +73,14 @@ def test_compact_paths_that_do_not_ascend(b2, torch, path, moved):
     kept = [i if j is None else j for i, j in enumerate(moved)]
     same, want, _ = compact_run(b2, torch, 2, 2, 64, 16, [10], [kept])
     assert (same == want).all() and (got == want).all()
+
+
+def test_compact_moves_what_lies_32_entries_behind_a_refused_one(b2, torch):
+    """A thread looks up entries i and i + 32: each is refused or moved for itself."""
+    path = [2 * i for i in range(8)] + list(range(20, 52))   # entry i of 8 and more is 12 + i
+    path[5] = path[4]
+    got, _, err = compact_run(b2, torch, 2, 2, 64, 16, [10], [path])
+    assert err == ERR_POSITION
+    path[5] = 5   # its own place: nothing to move
+    same, want, _ = compact_run(b2, torch, 2, 2, 64, 16, [10], [path])
+    assert (got == want).all()
