@@ -151,15 +151,21 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const b2_kv_plan_
         const int32_t page = lp < map[b] ? a.page_table[(size_t)b * a.pages_per_seq + lp]
                                          : a.free_pages[have - 1 - (int32_t)(fresh0[b] + lp - map[b])];
         const bool ok = page >= 0 && (uint32_t)page < a.pool_pages;
-        if (!ok) fault = B2_ERR_POSITION;
+        if (!ok) fault |= B2_ERR_POSITION;
+        uint32_t depth = i;
+        if (a.tree != nullptr) {
+            depth = (uint32_t)__popcll(a.tree[r]);
+            if (depth == 0) fault |= B2_ERR_TREE;
+            else --depth;
+        }
         a.row_item[r] = (int32_t)b;
-        a.row_pos[r] = (int32_t)(ctx[b] + (a.tree != nullptr ? (uint32_t)__popcll(a.tree[r]) - 1u : i));
+        a.row_pos[r] = (int32_t)(ctx[b] + depth);
         a.row_slot[r] = ok ? page * (int32_t)a.page_tokens + (int32_t)(at % a.page_tokens) : -1;
     }
     for (uint32_t k = blockIdx.x * kPlanThreads + tid; k < nfresh; k += stride) {
         const uint32_t b = plan_find(fresh0, a.batch, k);
         const int32_t page = a.free_pages[have - 1 - (int32_t)k];
-        if (page < 0 || (uint32_t)page >= a.pool_pages) fault = B2_ERR_POSITION;
+        if (page < 0 || (uint32_t)page >= a.pool_pages) fault |= B2_ERR_POSITION;
         a.page_table[(size_t)b * a.pages_per_seq + map[b] + k - fresh0[b]] = page;
     }
     if (fault) raise_error(a.err, fault);

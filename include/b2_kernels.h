@@ -444,7 +444,9 @@ int b2_rows_epilogue(const b2_rows_args *a, void *stream);
  * with cached tokens on no page, a negative length, more than B2_MAX_TREE rows
  * with a tree: B2_ERR_POSITION) changes no page table and gives every sequence
  * zero rows (row_start all 0, mapped_out and free_out as their inputs). A page
- * id outside [0, pool_pages) raises B2_ERR_POSITION and its rows get slot -1. */
+ * id outside [0, pool_pages) raises B2_ERR_POSITION and its rows get slot -1. An
+ * empty mask raises B2_ERR_TREE and its row gets depth 0; what else makes a mask
+ * no tree's is b2_tree_accept's to report. */
 typedef struct b2_kv_plan_args {
     uint32_t batch;              /* 1..B2_MAX_PLAN_BATCH */
     uint32_t max_rows;           /* length of the row arrays */

@@ -35,6 +35,24 @@ def torch():
     return torch
 
 
+# ---- b2_kv_plan, b2_rows_append -----------------------------------------------------------------------------
+
+
+def test_plan_mask_without_a_row(b2, torch):
+    """An empty mask is no tree's: reported, and the row's position is not before the new rows."""
+    for ctx in ([0, 20], [7, 0]):
+        c = plan_case(torch, ctx, [3, 4], 16, True)
+        want = plan_run(b2, torch, c)
+        c["masks"][1] = c["masks"][5] = 0
+        got = plan_run(b2, torch, c)
+        assert want["err"][0] == 0 and got["err"][0] == ERR_TREE
+        pos = want["pos"].copy()
+        pos[1], pos[5] = ctx[0], ctx[1]
+        assert (got["pos"] == pos).all()
+        for k in ("item", "slot", "start", "table", "mo", "fo"):
+            assert (got[k] == want[k]).all()
+
+
 # ---- b2_tree_accept, b2_kv_compact ----------------------------------------------------------------------------
 
 
