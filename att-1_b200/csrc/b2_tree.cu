@@ -446,7 +446,8 @@ extern "C" int b2_kv_plan(const b2_kv_plan_args *a, void *stream)
         return -1;  // positions and slots are int32
     if (a->batch > B2_MAX_PLAN_BATCH) return -9;
     const size_t smem = (size_t)a->batch * 4 * sizeof(uint32_t);
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    // (the default limit is 48 KB with the kernel's static shared memory, well below 16 KB)
+    if (smem > 32 * 1024 && cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  (int)(B2_MAX_PLAN_BATCH * 4 * sizeof(uint32_t))) != cudaSuccess)
         return -8;
     uint32_t blocks = (a->max_rows + kPlanRowsPerCta - 1) / kPlanRowsPerCta;

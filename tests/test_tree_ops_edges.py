@@ -38,6 +38,24 @@ def torch():
 # ---- b2_kv_plan, b2_rows_append -----------------------------------------------------------------------------
 
 
+BATCHES = """
+import sys
+sys.path[:0] = {path!r}
+import numpy as np, torch, att1_b200 as b2
+from test_tree_ops import plan_case, plan_check
+torch.cuda.init()
+for batch in (3055, 3056, 3070):
+    rng = np.random.default_rng(batch)
+    plan_check(b2, torch, plan_case(torch, rng.integers(0, 50, batch), rng.integers(0, 8, batch), 16, batch % 2 == 0, seed=batch))
+"""
+
+
+def test_plan_batches_at_the_shared_memory_limit():
+    """In a process of its own: a larger batch raises the kernel's limit for those after it."""
+    r = subprocess.run([sys.executable, "-c", BATCHES.format(path=sys.path)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+
+
 def test_plan_mask_without_a_row(b2, torch):
     """An empty mask is no tree's: reported, and the row's position is not before the new rows."""
     for ctx in ([0, 20], [7, 0]):
@@ -51,6 +69,48 @@ def test_plan_mask_without_a_row(b2, torch):
         assert (got["pos"] == pos).all()
         for k in ("item", "slot", "start", "table", "mo", "fo"):
             assert (got[k] == want[k]).all()
+
+
+def test_append_takes_as_many_rows_as_the_plan_before_it(b2, torch):
+    """Plan and append captured together, the second launched while the first runs: the rows in use are those of this replay."""
+    h, hkv, hd, page, batch, cap = 4, 2, 64, 16, 3, 24
+    pool = 12
+    L = b2.lib()
+    rng = np.random.default_rng(3)
+    y = dev(torch, rng.normal(0, 1, (cap, (h + 2 * hkv) * hd)), np.float32)
+    table, free = dev(torch, np.full((batch, 4), -1), np.int32), dev(torch, rng.permutation(pool), np.int32)
+    i32 = {k: torch.zeros(n, dtype=torch.int32, device="cuda") for k, n in dict(
+        ctx=batch, new=batch, mapped=batch, mo=batch, fo=1, start=batch + 1, item=cap, pos=cap, slot=cap, err=1).items()}
+    count = dev(torch, [pool], np.int32)
+    q = torch.zeros(cap, h * hd, device="cuda")
+    k, v = (torch.zeros(pool, hkv, page, hd, device="cuda") for _ in range(2))
+    plan = b2.KvPlanArgs(batch=batch, max_rows=cap, page_tokens=page, pages_per_seq=4, pool_pages=pool, ctx_len=p(i32["ctx"]),
+                         new_len=p(i32["new"]), mapped=p(i32["mapped"]), free_pages=p(free), free_count=p(count), page_table=p(table),
+                         mapped_out=p(i32["mo"]), free_out=p(i32["fo"]), row_start=p(i32["start"]), row_item=p(i32["item"]),
+                         row_pos=p(i32["pos"]), row_slot=p(i32["slot"]), err=p(i32["err"]), pdl=1)
+    app = b2.RowsAppendArgs(m=cap, y=p(y), y_stride=y.shape[1], q_rows=h * hd, q=p(q), q_stride=h * hd, slots=p(i32["slot"]),
+                            n_rows=i32["start"].data_ptr() + 4 * batch, kv=b2.KVLayout(p(k), p(v), None, page, 0, hkv, hd),
+                            pool_pages=pool, err=p(i32["err"]), pdl=1)
+
+    def step(stream):
+        b2.check("plan", L.b2_kv_plan(plan, stream))
+        b2.check("append", L.b2_rows_append(app, stream))
+
+    st = torch.cuda.Stream()
+    step(st.cuda_stream)
+    st.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        step(torch.cuda.current_stream().cuda_stream)
+    for new in ([1, 0, 2], [8, 8, 8], [0, 0, 0], [5, 1, 0], [2, 20, 2]):
+        i32["new"].copy_(dev(torch, new, np.int32))
+        q.fill_(7.25)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        n = sum(new)
+        assert int(i32["err"].item()) == 0 and int(i32["start"][batch].item()) == n
+        assert (q[:n] == y[:n, :h * hd]).all() and (q[n:] == 7.25).all()
 
 
 # ---- b2_tree_accept, b2_kv_compact ----------------------------------------------------------------------------
