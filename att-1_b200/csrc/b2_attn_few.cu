@@ -34,7 +34,8 @@ struct FewSmem {
     static constexpr uint32_t q_step = 2 * 32 * 16;                // hi and lo fragments of 16 rows x 16 dimensions
     static constexpr uint32_t off_q = kFewWarps * ring;
     static constexpr uint32_t off_cq = off_q + MT * (HD / 16) * q_step;  // [16 MT] f32: a row's score factor
-    static constexpr uint32_t off_mask = off_cq + 16 * MT * 4;          // [16 MT] u64
+    static constexpr uint32_t off_qt = off_cq + 16 * MT * 4;            // [16 MT] u32: bits of its largest |q|
+    static constexpr uint32_t off_mask = off_qt + 16 * MT * 4;          // [16 MT] u64
     static constexpr uint32_t off_hide = off_mask + 16 * MT * 8;        // [warps][4] u32: places on bad pages
     static constexpr uint32_t bytes = off_hide + kFewWarps * 4 * 4;
     // the warps' sums at the end, in the drained ring: values, then (maximum, sum), the CTA's last
@@ -87,6 +88,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
     const uint32_t split = blockIdx.x, kvh = blockIdx.y, item = blockIdx.z, hd = a.head_dim;
     uint8_t *ring = smem + warp * S::ring;
     float *cqs = reinterpret_cast<float *>(smem + S::off_cq);
+    uint32_t *tops = reinterpret_cast<uint32_t *>(smem + S::off_qt);
     uint64_t *masks = reinterpret_cast<uint64_t *>(smem + S::off_mask);
     uint32_t *hides = reinterpret_cast<uint32_t *>(smem + S::off_hide) + warp * 4;
     pdl_wait();
@@ -176,6 +178,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
         }
         if (lane == 0) {
             cqs[r] = bad ? NAN : pow2i(e) * p.scale;
+            tops[r] = bad ? 0 : top;
             masks[r] = mine && a.tree != nullptr ? a.tree[r0 + tok] : 0;
         }
     }
@@ -189,6 +192,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
         m[i] = -INFINITY;
         l[i] = 0.0f;
     }
+    const bool far = rows_far(tops[lane % (16 * MT)], p.reach);
     float acc[MT][4 * QG][4];  // column (q, i): dimensions 32 q + 4 col + i, col 2 t4 and 2 t4 + 1
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -284,14 +288,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
         fill();  // into the slot just read
         // ---- softmax: a lane holds columns 8 nt + 2 t4, + 1 of its rows ----
         const bool masked = p0 + kFewUnit > ctx || none != 0 || kbad != 0;
-        if (__builtin_expect(kwide, 0)) {
+        const bool apart = kwide || ke > 0 || far;  // scores rounded before the maximum is subtracted
+        if (__builtin_expect(apart, 0)) {
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
-                    const float f = pow2i(__shfl_sync(0xffffffffu, kpe, 8 * nt + 2 * t4 + v));
+                    const int own = __shfl_sync(0xffffffffu, kpe, 8 * nt + 2 * t4 + v), e = kwide ? own : ke;
 #pragma unroll
-                    for (int i = 0; i < 2 * MT; ++i) s[i / 2][nt][(i & 1) * 2 + v] = s[i / 2][nt][(i & 1) * 2 + v] * cq[i] * f;
+                    for (int i = 0; i < 2 * MT; ++i) s[i / 2][nt][(i & 1) * 2 + v] = place_score(s[i / 2][nt][(i & 1) * 2 + v], cq[i], e);
                 }
         }
         float corr[2 * MT];
@@ -299,7 +304,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i) {
             float *s0 = &s[i / 2][0][(i & 1) * 2], *s1 = &s[i / 2][1][(i & 1) * 2];
-            const float cqk = kwide ? 1.0f : score_factor(cq[i], ke);
+            const float cqk = apart ? 1.0f : score_factor(cq[i], ke);
             if (masked) {
                 const uint32_t vis = visible((i / 2) * 16 + g8 + (i & 1) * 8, p0) & ~none;
 #pragma unroll
@@ -315,7 +320,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // kept while it grows by less than kRowsSlack, so that the sums are seldom rescaled
             const float m_new = top > m[i] + kRowsSlack ? top : m[i];
-            const float m_use = m_new == -INFINITY ? 0.0f : m_new, shift = kRowsP - m_use;
+            const float m_use = m_new == -INFINITY ? 0.0f : m_new, shift = apart ? kRowsP : kRowsP - m_use;
+            if (__builtin_expect(apart, 0)) s0[0] -= m_use, s0[1] -= m_use, s1[0] -= m_use, s1[1] -= m_use;
             corr[i] = ex2(m[i] - m_use);
             rescale |= m_new != m[i];
             m[i] = m_new;

@@ -60,7 +60,8 @@ struct LaidSmem {
     static constexpr uint32_t off_v = off_k + k_stages * 2 * P::k_half;
     static constexpr uint32_t off_m = off_v + v_stages * P::v_tile;  // [kLaidMarks][2] marks of a tile
     static constexpr uint32_t off_cq = off_m + kLaidMarks * 2 * TileMarks::bytes;  // [128] f32: the rows' score factors
-    static constexpr uint32_t off_ri = off_cq + kRowsM * 4;         // [4][128] (f32, f32): a tile's maximum and factor per row
+    static constexpr uint32_t off_qt = off_cq + kRowsM * 4;         // [128] u32: bits of their largest |q|
+    static constexpr uint32_t off_ri = off_qt + kRowsM * 4;         // [4][128] (f32, f32): a tile's maximum and factor per row
     static constexpr uint32_t off_l = off_ri + 4 * kRowsM * 8;      // [group][128] (f32, f32): maximum and sum at the end
     static constexpr uint32_t off_bar = off_l + 2 * kRowsM * 8;
     static constexpr uint32_t bytes = off_bar + 8 * (2 * k_stages + 2 * v_stages + 2 + 2 * 2 + 4) + 16;
@@ -116,11 +117,11 @@ __global__ void __launch_bounds__(kLayWarps * 32) attn_rows_lay_kernel(const Row
 // A block's rows of q as operand A, in two steps of eight warps w with a barrier between:
 // whole rows, coalesced, into hi and lo images in shared memory (128 rows of HD f16 each;
 // 16-byte pieces of a row are permuted by it, so that a thread per row reads without
-// conflicts), with the rows' score factors; then a thread's row into tensor memory, the
-// dimensions of one half.
+// conflicts), with the rows' score factors and largest |q|; then a thread's row into
+// tensor memory, the dimensions of one half.
 template <int HD>
 __device__ __forceinline__ void stage_q(const RowsParams &p, uint32_t w, uint32_t r0, uint32_t kvh, uint32_t first, uint32_t live, uint8_t *hi,
-                                        uint8_t *lo, float *cqs)
+                                        uint8_t *lo, float *cqs, uint32_t *tops)
 {
     constexpr uint32_t kAhead = 8;  // rows asked for at a time
     const b2_attn_rows_args &a = p.a;
@@ -145,7 +146,10 @@ __device__ __forceinline__ void stage_q(const RowsParams &p, uint32_t w, uint32_
             const int e = bad ? 0 : top_exp(top);
             const float sc = pow2i(-e);
             if (bad) f[i] = make_float4(0, 0, 0, 0);
-            if (lane == 0) cqs[r] = bad ? NAN : pow2i(e) * p.scale;
+            if (lane == 0) {
+                cqs[r] = bad ? NAN : pow2i(e) * p.scale;
+                tops[r] = bad ? 0 : top;
+            }
             if (4 * lane < HD) {
                 uint2 h2, l2;
                 split_f16(f[i].x * sc, f[i].y * sc, h2.x, l2.x);
@@ -417,13 +421,16 @@ __global__ void __launch_bounds__(kLaidThreads, 1) attn_laid_kernel(const RowsPa
         // ---- softmax of every other tile: row r ----
         const uint32_t g = warp / kLaidSoftWarps, qt = warp & 3, r = qt * 32 + lane;
         uint8_t *q_hi = smem + S::off_k + (NK - 1) * 2 * P::k_half, *q_lo = q_hi + P::k_half;
-        stage_q<HD>(p, warp, r0, kvh, blk * kRowsM, live, q_hi, q_lo, cqs);
+        stage_q<HD>(p, warp, r0, kvh, blk * kRowsM, live, q_hi, q_lo, cqs, reinterpret_cast<uint32_t *>(smem + S::off_qt));
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (qt < nq) {
             const bool mine = r < live;
             const uint32_t tok = mine ? (blk * kRowsM + r) / p.group : 0;
             const uint32_t lanes = (qt * 32) << 16;
-            const float cq = mine ? cqs[r] : 0.0f;  // score of a row: dot * K scale * cq, in powers of two
+            // score of a row: dot * K scale * cq, in powers of two; the sign says whether the warp's rows
+            // are far (a register of its own, held over the loop, cost 1.5 percent)
+            const bool far = rows_far(mine ? reinterpret_cast<const uint32_t *>(smem + S::off_qt)[r] : 0, p.reach);
+            const float cq = copysignf(mine ? cqs[r] : 0.0f, far ? -1.0f : 1.0f);
             put_q<HD>(tm_q + lanes, g, r, q_hi, q_lo);
             tmem_wait_st();
             fence_proxy_async();  // (a copy writes there next)
@@ -433,8 +440,8 @@ __global__ void __launch_bounds__(kLaidThreads, 1) attn_laid_kernel(const RowsPa
             const uint64_t mask = mine && a.tree != nullptr ? a.tree[r0 + tok] : 0;
             float m = -INFINITY, l = 0.0f;
             bool ok = true;
-            // One tile; those with units of different scale or marked places have a copy of the code
-            // of their own.
+            // One tile; those with units of different scale, marked places or scores past 2^23 have
+            // a copy of the code of their own.
             auto tile = [&](uint32_t j, auto rare, const uint8_t *marks) {
                 constexpr bool RARE = decltype(rare)::value;
                 const uint32_t *ks = reinterpret_cast<const uint32_t *>(marks), *vs = reinterpret_cast<const uint32_t *>(marks + TileMarks::off_vm);
@@ -461,7 +468,7 @@ __global__ void __launch_bounds__(kLaidThreads, 1) attn_laid_kernel(const RowsPa
                 if (RARE) {
 #pragma unroll
                     for (int k = 0; k < 64; ++k) {
-                        s[k] = s[k] * cq * pow2i(exp_of(ks, ke, k));
+                        s[k] = place_score(s[k], fabsf(cq), exp_of(ks, ke, k));
                         if (ks[k / 8] >> (k & 7) & 1) s[k] = NAN;
                     }
                 }
@@ -482,7 +489,12 @@ __global__ void __launch_bounds__(kLaidThreads, 1) attn_laid_kernel(const RowsPa
                 const float m_use = m_new == -INFINITY ? 0.0f : m_new;
                 const float corr = ex2(m - m_use);
                 m = m_new;
-                const uint64_t cq2 = pair(cqk, cqk), sh2 = pair(kRowsP - m_use, kRowsP - m_use);
+                const float shift = RARE ? kRowsP : kRowsP - m_use;
+                if (RARE) {
+#pragma unroll
+                    for (int k = 0; k < 64; ++k) s[k] -= m_use;
+                }
+                const uint64_t cq2 = pair(cqk, cqk), sh2 = pair(shift, shift);
                 uint64_t sum = 0;
 #pragma unroll
                 for (int k = 0; k < 64; k += 2) {
@@ -528,7 +540,7 @@ __global__ void __launch_bounds__(kLaidThreads, 1) attn_laid_kernel(const RowsPa
                 tc_fence_after();
                 const uint8_t *marks = smem + S::off_m + (i % kLaidMarks * 2 + g) * TileMarks::bytes;
                 const uint32_t *ks = reinterpret_cast<const uint32_t *>(marks);
-                if (units_plain(ks) && units_plain(ks + 8)) tile(j, std::false_type(), marks);
+                if (units_plain(ks) && ks[0] <= meta_of_exp(0) && __float_as_int(cq) >= 0 && units_plain(ks + 8)) tile(j, std::false_type(), marks);
                 else tile(j, std::true_type(), marks);
             }
             ends[g * kRowsM + r] = make_float2(m, l);

@@ -292,6 +292,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
             const uint32_t tok = mine ? m_row / p.group : 0, head = kvh * p.group + (mine ? m_row % p.group : 0);
             const uint32_t lanes = (qt * 32) << 16;
             float cq;  // score of a row: dot * K scale * cq, in powers of two
+            bool far;  // the warp's rows
             {
                 const float *src = a.q + (size_t)(r0 + tok) * a.q_stride + (size_t)head * hd;
                 uint32_t top = 0;
@@ -303,6 +304,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 const int e = bad ? 0 : top_exp(top);
                 const float sc = pow2i(-e);
                 cq = bad ? NAN : pow2i(e) * p.scale;
+                far = rows_far(bad ? 0 : top, p.reach);
 #pragma unroll
                 for (uint32_t c = 0; c < HD / 2; c += 32) {  // 32 dimensions: 16 columns of hi, 16 of lo
                     uint32_t hi[16], lo[16];
@@ -363,9 +365,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 }
             };
             auto visible = [&](uint32_t key0) { return rows_visible(a.tree != nullptr, mask, tok, ctx, places, key0); };
-            // One tile. Units of K or V of different scale and marked places are rare and cost the
-            // others nothing: they have a copy of the code of their own (in one, the branches and
-            // what they keep in registers slowed every tile by 5 to 9 percent).
+            // One tile. Units of K or V of different scale, marked places and scores that may pass
+            // 2^23 are rare and cost the others next to nothing: they have a copy of the code of
+            // their own (in one, the branches and what they keep in registers slowed every tile by
+            // 5 to 9 percent).
             auto tile = [&](uint32_t j, auto rare, const uint4 &km, const uint4 &va, const uint4 &vb) {
                 constexpr bool RARE = decltype(rare)::value;
                 const uint32_t mt = j % kRowsMeta, vt = j & 1, key0 = (t0 + j) * kRowsKeys + half * 32;
@@ -390,12 +393,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 sum16(16);
                 float cqk = score_factor(cq, meta_exp(km.x));
                 uint32_t vis = key0 + 32 > ctx ? visible(key0) : 0xFFFFFFFFu;
-                if (RARE && !meta_plain(km)) {
+                if (RARE) {
                     const uint32_t bad = meta_bytes(km, 0);
                     vis &= ~meta_bytes(km, 8);
 #pragma unroll
                     for (int k = 0; k < 32; ++k) {
-                        s[k] = s[k] * cq * pow2i(exp_of(kmeta + mt * 8, kexp + mt * kRowsKeys, half * 32 + k));
+                        s[k] = place_score(s[k], cq, exp_of(kmeta + mt * 8, kexp + mt * kRowsKeys, half * 32 + k));
                         if (bad >> k & 1) s[k] = NAN;
                     }
                     cqk = 1.0f;
@@ -422,7 +425,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 const float m_use = m_new == -INFINITY ? 0.0f : m_new;
                 const float corr = ex2(m - m_use);
                 m = m_new;
-                const uint64_t cq2 = pair(cqk, cqk), sh2 = pair(kRowsP - m_use, kRowsP - m_use);
+                const float shift = RARE ? kRowsP : kRowsP - m_use;
+                if (RARE) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) s[k] -= m_use;
+                }
+                const uint64_t cq2 = pair(cqk, cqk), sh2 = pair(shift, shift);
                 uint64_t sum = 0;
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
@@ -473,7 +481,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                 tc_fence_after();
                 const uint4 km = *reinterpret_cast<const uint4 *>(kmeta + (j % kRowsMeta) * 8 + half * 4),
                             va = *reinterpret_cast<const uint4 *>(vmeta + (j & 1) * 8), vb = *reinterpret_cast<const uint4 *>(vmeta + (j & 1) * 8 + 4);
-                if (meta_plain(km) && meta_plain(va) && meta_plain(vb) && va.x == vb.x) tile(j, std::false_type(), km, va, vb);
+                if (meta_plain(km) && km.x <= meta_of_exp(0) && !far && meta_plain(va) && meta_plain(vb) && va.x == vb.x) tile(j, std::false_type(), km, va, vb);
                 else tile(j, std::true_type(), km, va, vb);
             }
             wait(&o_full[(nt - 1) & 1], (nt - 1) / 2);
@@ -701,6 +709,7 @@ extern "C" int b2_attn_rows(const b2_attn_rows_args *a, void *stream)
     p.laid = (uint8_t *)a->scratch;
     p.part = (float *)((uint8_t *)a->scratch + (size_t)a->batch * a->n_kv_heads * p.pairs * attn_laid_pair(a->head_dim));
     p.scale = (float)(1.4426950408889634 / sqrt((double)a->head_dim));
+    p.reach = p.scale * (float)a->head_dim;
     const cudaStream_t st = (cudaStream_t)stream;
     if (few) {
         if (attn_few_launch(p, st) != cudaSuccess) return -8;

@@ -20,7 +20,7 @@ struct RowsParams {
     uint32_t blocks, splits;  // blocks per (item, KV head), splits of their places
     uint32_t pairs;           // K and V are laid out as operands first: pairs of tiles of an (item, KV head), else 0
     uint8_t *laid;            // [item][KV head][pair]
-    float scale;              // log2(e) / sqrt(head_dim)
+    float scale, reach;       // log2(e) / sqrt(head_dim), and head_dim times that
     float *part;              // splits to be joined by a kernel: [item][KV head][block][split][rows of a block][head_dim + 4]:
                               // maximum (log2), sum, -, -, weighted values
 };
@@ -134,6 +134,7 @@ __device__ __forceinline__ uint32_t unit_meta(int e, bool wide, uint32_t hidden,
 {
     return (uint32_t)wide << 24 | (uint32_t)(e + 128) << 16 | hidden << 8 | bad;
 }
+__host__ __device__ constexpr uint32_t meta_of_exp(int e) { return (uint32_t)(e + 128) << 16; }  // nothing marked
 __device__ __forceinline__ int meta_exp(uint32_t m) { return (int)(m >> 16 & 0xFF) - 128; }
 // byte i of the result: (m_i >> shift) & 0xFF
 __device__ __forceinline__ uint32_t meta_bytes(const uint4 &m, uint32_t shift)
@@ -217,6 +218,19 @@ __device__ __forceinline__ float score_factor(float cq, int e)
     const float f = cq * pow2i(e);
     return f == 0.0f ? 1e-38f : f;
 }
+
+// Scores and their distance to the maximum come from one fused multiply-add, of which the
+// maximum is a rounding: below 2^23 they differ by less than 1/2, and a weight does not pass
+// f16's range. Beyond, scores are rounded first (place_score), and the maximum subtracted
+// from that: for K of exponents above 0 (2^12 and more), and where a warp's rows are far,
+// their largest |q_i| (its bits) times head_dim times 2^12, scaled like a score, at 2^23.
+__device__ __forceinline__ bool rows_far(uint32_t top, float reach)
+{
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, top)) * reach >= 2048.0f;
+}
+// The rounded score of a place of exponent e, in two steps of e: the row's factor and e may
+// both be far from 1, and s * cq or cq * 2^e out of range where the score is not.
+__device__ __forceinline__ float place_score(float s, float cq, int e) { return s * (cq * pow2i(e / 2)) * pow2i(e - e / 2); }
 
 // All lanes wait; false for the whole warp if any gave up.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase, int32_t *err)

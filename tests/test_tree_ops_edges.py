@@ -35,6 +35,82 @@ def torch():
     return torch
 
 
+def exact(s, hide=()):
+    """Outputs in float64 without the places of `hide`; sum_j p_j |v_j|; the bound of a weight's relative error; the least gap
+    of a row's two best scores."""
+    out = np.zeros((s.rows, s.h, s.hd))
+    size, rel, gap = np.zeros_like(out), 0.0, np.inf
+    g, scale = s.h // s.hkv, 1 / np.sqrt(s.hd)
+    for b in range(s.batch):
+        t = int(s.ctx[b] + s.new[b])
+        pg, off = s.table[b, np.arange(t) // s.page], np.arange(t) % s.page
+        K, V = s.k[pg, :, off].astype(np.float64), s.v[pg, :, off].astype(np.float64)
+        for i in range(int(s.new[b])):
+            at = [j for j in s.sees(b, i) if j not in hide]
+            q = s.q[s.start[b] + i, :s.h * s.hd].astype(np.float64).reshape(s.hkv, g, s.hd)
+            x = np.einsum("hgd,thd->hgt", q, K[at]) * scale
+            top = np.sort(x, -1)
+            gap = min(gap, (top[..., -1] - top[..., -2]).min())
+            w = np.exp(x - x.max(-1, keepdims=True))
+            w /= w.sum(-1, keepdims=True)
+            r = s.start[b] + i
+            out[r] = np.einsum("hgt,thd->hgd", w, V[at]).reshape(s.h, s.hd)
+            size[r] = np.einsum("hgt,thd->hgd", w, np.abs(V[at])).reshape(s.h, s.hd)
+            a = np.einsum("hgd,thd->hgt", np.abs(q), np.abs(K[at])).max() * scale
+            rel = max(rel, 2 * (a * 2.0 ** -21 + scale * 2.0 ** -25 * (np.abs(q).sum(-1).max() + np.abs(K[at]).sum(-1).max())))
+    return out, size, rel, gap
+
+
+# ---- attention --------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("size_q,size_k", [(10, 12), (12, 12), (11, 14), (13, 14), (16, 15), (30, 30), (60, -25), (-25, 60)])
+@pytest.mark.parametrize("h,hkv,hd,new", FEW + ROWS + LAID)
+def test_attn_scores_of_any_size(b2, torch, h, hkv, hd, new, size_q, size_k):
+    """Scores of 2^23 to 2^61: where one place is ahead by more than they can be off, its V comes out."""
+    s = Scene(torch, h, hkv, hd, 16, [61], [new], seed=24)
+    s.q *= np.float32(2.0 ** size_q)
+    s.k *= np.float32(2.0 ** size_k)
+    ref, _, _, gap = exact(s)
+    assert gap > 0
+    t = 61 + new
+    pg, off = s.table[0, np.arange(t) // 16], np.arange(t) % 16
+    got, err = s.run(b2)
+    assert err == 0
+    clear = 0
+    for i in range(new):
+        at = s.sees(0, i)
+        for hh in range(h):
+            q, K = s.q[i, hh * hd:(hh + 1) * hd].astype(np.float64), s.k[pg[at], hh // (h // hkv), off[at]].astype(np.float64)
+            x, a = K @ q / np.sqrt(hd), (np.abs(K) @ np.abs(q)).max() / np.sqrt(hd)
+            if np.diff(np.sort(x)[-2:])[0] > 2 * a * 2.0 ** -21 + 32:   # the second's weight is below 2^-46
+                clear += 1
+                assert np.abs(got[i, hh] - ref[i, hh]).max() <= 2.0 ** -19 * np.nanmax(np.abs(s.v))
+    assert clear > 0.95 * new * h
+
+
+@pytest.mark.parametrize("h,hkv,hd,new", FEW + ROWS + LAID)
+def test_attn_scores_in_range_of_operands_far_from_one(b2, torch, h, hkv, hd, new):
+    """q of 2^126 and K of 2^-90, some places 2^-98 and one hidden from some rows 2^13: scores of 2^36, one weight takes all."""
+    s = Scene(torch, h, hkv, hd, 16, [61], [new], seed=23)
+    t = 61 + new
+    victim = 3
+    s.q = (np.sign(s.q) * np.float32(2.0 ** 126) * (1 + np.abs(s.q) / 16)).astype(np.float32)
+    s.k *= np.float32(2.0 ** -90)
+    for j in range(t):
+        if j % 24 < 8:
+            pg, off = s.place(0, j)
+            s.k[pg, :, off] *= np.float32(2.0 ** -8)
+    pg, off = s.place(0, 61 + victim)
+    s.k[pg, :, off] = np.sign(s.k[pg, :, off]) * 2.0 ** 13
+    rows = [i for i in range(new) if not s.masks[i] >> victim & 1]
+    assert rows and np.isfinite(s.q).all()
+    ref, _, _, gap = exact(s, hide=(61 + victim,))
+    assert gap > 2.0 ** 20   # against an error of about 2^37 2^-21
+    got, _ = s.run(b2)
+    assert np.abs(got[rows] - ref[rows]).max() <= 2.0 ** -19 * np.nanmax(np.abs(s.v))
+
+
 # ---- b2_kv_plan, b2_rows_append -----------------------------------------------------------------------------
 
 
