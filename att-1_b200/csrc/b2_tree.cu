@@ -192,7 +192,8 @@ __global__ void __launch_bounds__(2 * kAppendThreads) rows_append_kernel(const b
     const uint32_t col = threadIdx.x % cols, hg = threadIdx.x / cols;
     const uint32_t qh = a.q_rows / hd, hkv = a.kv.n_kv_heads, heads = qh + 2 * hkv;
     const uint32_t h0 = blockIdx.x * heads_per_part, h1 = min(heads, h0 + heads_per_part);
-    const uint32_t m = a.n_rows != nullptr ? (uint32_t)min(max(__ldg(a.n_rows), 0), (int32_t)min(a.m, 0x7FFFFFFFu)) : a.m;
+    // (not a read-only load: the kernel before may write it while this one is resident)
+    const uint32_t m = a.n_rows != nullptr ? (uint32_t)min(max(*a.n_rows, 0), (int32_t)min(a.m, 0x7FFFFFFFu)) : a.m;
     const uint32_t slots = a.pool_pages * a.kv.page_tokens;
     if (hg >= hgroups) return;
     for (uint32_t n = blockIdx.y; n < m; n += gridDim.y) {
