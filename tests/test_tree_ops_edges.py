@@ -64,6 +64,110 @@ def exact(s, hide=()):
 # ---- attention --------------------------------------------------------------------------------------------
 
 
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("victim", [1, 2, 4, 6])
+@pytest.mark.parametrize("h,hkv,hd,new", FEW[:2])
+def test_attn_few_rows_masked_places_may_hold_anything(b2, torch, h, hkv, hd, new, victim, which, bad):
+    """Places 38 to 43: both halves of a unit of 16, and neighbouring columns of a lane."""
+    s = Scene(torch, h, hkv, hd, 16, [37], [new], seed=13)
+    ref = s.reference()
+    pg, off = s.place(0, 37 + victim)
+    getattr(s, which)[pg, hkv - 1, off, 5] = bad
+    got, err = s.run(b2)
+    first = (hkv - 1) * (h // hkv)   # heads of the KV head that holds it
+    seen = [bool(s.masks[i] >> victim & 1) for i in range(new)]
+    assert any(seen) and not all(seen) and err == ERR_NONFINITE
+    for i in range(new):
+        assert np.abs(got[i, :first] - ref[i, :first]).max(initial=0) <= ATTN_TOL * 5
+        if seen[i]:
+            assert np.isnan(got[i, first:]).all()
+        else:
+            assert np.abs(got[i, first:] - ref[i, first:]).max() <= ATTN_TOL * 5
+
+
+@pytest.mark.parametrize("at", [0, 3, 20, 31, 36])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("h,hkv,hd,new", FEW)
+def test_attn_few_rows_nonfinite_cached_place(b2, torch, h, hkv, hd, new, which, at):
+    """A cached place is seen by every row."""
+    s = Scene(torch, h, hkv, hd, 16, [37], [new], seed=14)
+    ref = s.reference()
+    pg, off = s.place(0, at)
+    getattr(s, which)[pg, 0, off, hd - 1] = np.nan
+    got, err = s.run(b2)
+    assert err == ERR_NONFINITE and np.isnan(got[:, :h // hkv]).all()
+    assert np.abs(got[:, h // hkv:] - ref[:, h // hkv:]).max(initial=0) <= ATTN_TOL * 5
+
+
+@pytest.mark.parametrize("big", [3e3, 1e5, 1e10, 1e30, 3e38])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("victim", [1, 2, 4, 6])
+@pytest.mark.parametrize("h,hkv,hd,new", FEW[:2])
+def test_attn_few_rows_hidden_place_takes_no_precision(b2, torch, h, hkv, hd, new, victim, which, big):
+    s = Scene(torch, h, hkv, hd, 16, [37], [new], seed=13)
+    ref = s.reference()
+    pg, off = s.place(0, 37 + victim)
+    getattr(s, which)[pg, :, off] = big * np.sign(getattr(s, which)[pg, :, off])
+    got, _ = s.run(b2)
+    hidden = [i for i in range(new) if not s.masks[i] >> victim & 1]
+    assert hidden
+    assert np.abs(got[hidden] - ref[hidden]).max() <= ATTN_TOL * 5
+
+
+@pytest.mark.parametrize("at", [5, 12, 20, 31, 36])
+@pytest.mark.parametrize("h,hkv,hd,new", FEW)
+def test_attn_few_rows_place_of_no_weight_takes_no_precision(b2, torch, h, hkv, hd, new, at):
+    """A cached place whose K is 2^14 times the others' in one direction and whose V is 2^40."""
+    s = Scene(torch, h, hkv, hd, 16, [37], [new], seed=16)
+    pg, off = s.place(0, at)
+    s.k[pg, :, off] = 0
+    s.k[pg, :, off, 3] = 2.0 ** 14
+    s.v[pg, :, off] = 2.0 ** 40
+    q = s.q[:s.rows, :h * hd].reshape(s.rows, h, hd)
+    q[:, :, 3] = np.where(q[:, :, 3] > 0, 1, -1)  # scores of +-2^14 / sqrt(hd)
+    got, err = s.run(b2)
+    drawn = q[:, :, 3] > 0
+    assert err == 0 and drawn.any() and not drawn.all()
+    assert (np.abs(got[drawn] - 2.0 ** 40) <= ATTN_TOL * 2.0 ** 40).all()
+    others = exact(s, hide=(at,))[0]
+    assert np.abs(got[~drawn] - others[~drawn]).max() <= ATTN_TOL * 5
+
+
+@pytest.mark.parametrize("growing", [True, False, None])
+@pytest.mark.parametrize("h,hkv,hd,new", FEW + ROWS + LAID)
+def test_attn_saturated_softmax(b2, torch, h, hkv, hd, new, growing):
+    """Scores past +-60, every place's K times a power of two of its own from 2^-6 to 2^3, growing along the places (the maximum
+    rises from tile to tile and the sums are rescaled), falling, or in no order."""
+    s = Scene(torch, h, hkv, hd, 16, [300], [new], seed=21)
+    t = 300 + new
+    size = np.floor(np.arange(t) * 9.99 / t).astype(int) - 6
+    if growing is None:
+        size = np.random.default_rng(5).permutation(size)
+    elif not growing:
+        size = size[::-1]
+    pg, off = s.table[0, np.arange(t) // 16], np.arange(t) % 16
+    s.k[pg, :, off] *= np.ldexp(np.float32(1), size)[:, None, None]
+    s.q *= np.float32(6)
+    ref, mean, rel, _ = exact(s)
+    top = np.einsum("hgd,thd->hgt", s.q[0, :h * hd].reshape(hkv, h // hkv, hd), s.k[pg[:300], :, off[:300]]) / np.sqrt(hd)
+    assert np.abs(top).max() > 60
+    got, err = s.run(b2)
+    assert err == 0
+    assert (np.abs(got - ref) <= (rel + 2.0 ** -19) * mean.max(-1, keepdims=True) + 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("h,hkv,hd,new", FEW + ROWS + LAID)
+def test_attn_small_channels(b2, torch, h, hkv, hd, new):
+    """Dimension d of V times 2^-(d mod 16): every dimension keeps its own bound, 2^-25 of 1 at the finest."""
+    s = Scene(torch, h, hkv, hd, 16, [150], [new], seed=22)
+    s.v *= np.ldexp(np.float32(1), -(np.arange(hd) % 16))
+    ref, mean, rel, _ = exact(s)
+    got, err = s.run(b2)
+    assert err == 0
+    assert (np.abs(got - ref) <= (rel + 2.0 ** -19) * mean + 2.0 ** -24).all()
+
+
 @pytest.mark.parametrize("size_q,size_k", [(10, 12), (12, 12), (11, 14), (13, 14), (16, 15), (30, 30), (60, -25), (-25, 60)])
 @pytest.mark.parametrize("h,hkv,hd,new", FEW + ROWS + LAID)
 def test_attn_scores_of_any_size(b2, torch, h, hkv, hd, new, size_q, size_k):
@@ -238,3 +342,27 @@ def test_compact_moves_what_lies_32_entries_behind_a_refused_one(b2, torch):
     path[5] = 5   # its own place: nothing to move
     same, want, _ = compact_run(b2, torch, 2, 2, 64, 16, [10], [path])
     assert (got == want).all()
+
+
+def test_compact_pools_past_32_bits_of_places(b2, torch):
+    """K and V in one buffer of more than 2^32 places, V's pages one behind K's: no place belongs to both."""
+    page, n = 1 << 16, (1 << 16) + 4
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("not enough device memory free")
+    pool = torch.empty(n, page, 4, device="cuda")
+    pages = [n - 3, 2]
+    table = dev(torch, [pages], np.int32)
+    rows = torch.arange(80, dtype=torch.float32, device="cuda").reshape(2, 10, 4) + 1
+    for x in (0, 1):   # places page - 3 .. page + 6 of the sequence
+        pool[pages[0] + x, page - 3:], pool[pages[1] + x, :7] = rows[x, :3], rows[x, 3:]
+    path = torch.full((1, 64), -1, dtype=torch.int32, device="cuda")
+    path[0, :4] = dev(torch, [0, 2, 5, 9], np.int32)
+    kv = (b2.KVLayout * 1)(b2.KVLayout(p(pool), pool[1].data_ptr(), p(table), page, 2, 1, 4))
+    d = dict(ctx=dev(torch, [page - 3], np.int32), count=dev(torch, [4], np.int32), err=torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert b2.lib().b2_kv_compact(b2.KvCompactArgs(n_layers=1, layers=kv, pool_pages=n - 1, batch=1, ctx_len=p(d["ctx"]), path=p(path),
+                                                   count=p(d["count"]), err=p(d["err"])), None) == 0
+    torch.cuda.synchronize()
+    assert int(d["err"].item()) == 0
+    for x in (0, 1):
+        assert (pool[pages[0] + x, page - 3:] == rows[x, [0, 2, 5]]).all()
+        assert (pool[pages[1] + x, 0] == rows[x, 9]).all() and (pool[pages[1] + x, 1:7] == rows[x, 4:]).all()
