@@ -24,7 +24,8 @@ cpu_baseline: the reference CPU implementation (compiled from its sources,
        oracle/_ref) on a bounded sample of the same workload, all host cores
        for its matmuls.
 
---impl reference runs only that reference CPU measurement (rank 0).
+--impl reference runs only that reference CPU measurement (rank 0). Where the
+compiled reference is missing it prints why, and cpu_baseline says the same.
 Under torchrun (N>1) ranks run tensor-parallel shards when the build
 supports it; the JSON line reports whole-job tokens/s (max time over ranks).
 """
@@ -124,6 +125,16 @@ class ClockSampler:
 # ---------------------------------------------------------------------------------------------
 
 REF_SHIPPED = "libatt1ref_shipped.so"   # the reference Makefile's flags (no -O)
+
+
+def reference_missing():
+    """Why the reference CPU path cannot be timed here, None where it can."""
+    sys.path.insert(0, os.path.join(ROOT, "oracle"))
+    import oracle as O
+    if os.path.exists(O.REF_SO):
+        return None
+    return (f"{os.path.relpath(O.REF_SO, ROOT)} not built: the oracle's Makefile compiles it from the reference's sources "
+            "(ATT1_REFERENCE_DIR)")
 
 
 def reference_cpu_sample(ctx, steps=2, warmup=1, threads=None, lib=None):
@@ -617,7 +628,10 @@ def run_b200(args, rank, world, local_rank):
     out = None
     if rank == 0:
         cpu = None
-        if world == 1 and not args.no_cpu:
+        missing = reference_missing()
+        if world == 1 and not args.no_cpu and missing:
+            cpu = {"unavailable": missing}
+        elif world == 1 and not args.no_cpu:
             r = reference_cpu_sample(ctx)
             cpu = {"value": r["value"], "unit": "tokens/s", "cores": r["cores"], "kind": "reference",
                    "sample": r["sample"], "extrapolated": True}
@@ -657,6 +671,9 @@ def run_reference(args, rank):
     steps reported are the steps timed on each sample model."""
     if rank != 0:
         return None
+    missing = reference_missing()
+    if missing:
+        return {"impl": "reference", "unavailable": missing}
     steps = max(1, args.steps)
     r = reference_cpu_sample(args.ctx, steps=steps, warmup=max(0, args.warmup))
     v = r["value"]
