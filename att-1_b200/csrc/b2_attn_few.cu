@@ -24,7 +24,7 @@
 
 namespace b2 {
 
-constexpr int MT = kFewRows / 16;  // MMA tiles of rows
+static_assert(kFewRows == 16, "one MMA tile of rows");
 
 template <int HD>
 struct FewSmem {
@@ -33,14 +33,14 @@ struct FewSmem {
     static constexpr uint32_t ring = slots * slot;
     static constexpr uint32_t q_step = 2 * 32 * 16;                // hi and lo fragments of 16 rows x 16 dimensions
     static constexpr uint32_t off_q = kFewWarps * ring;
-    static constexpr uint32_t off_cq = off_q + MT * (HD / 16) * q_step;  // [16 MT] f32: a row's score factor
-    static constexpr uint32_t off_qt = off_cq + 16 * MT * 4;            // [16 MT] u32: bits of its largest |q|
-    static constexpr uint32_t off_mask = off_qt + 16 * MT * 4;          // [16 MT] u64
-    static constexpr uint32_t off_hide = off_mask + 16 * MT * 8;        // [warps][4] u32: places on bad pages
+    static constexpr uint32_t off_cq = off_q + (HD / 16) * q_step;  // [16] f32: a row's score factor
+    static constexpr uint32_t off_qt = off_cq + kFewRows * 4;       // [16] u32: bits of its largest |q|
+    static constexpr uint32_t off_mask = off_qt + kFewRows * 4;     // [16] u64
+    static constexpr uint32_t off_hide = off_mask + kFewRows * 8;   // [warps][4] u32: places on bad pages
     static constexpr uint32_t bytes = off_hide + kFewWarps * 4 * 4;
     // the warps' sums at the end, in the drained ring: values, then (maximum, sum), the CTA's last
-    static constexpr uint32_t off_o = 0, off_ml = kFewWarps * 16 * MT * HD * 4;
-    static_assert(off_ml + (kFewWarps + 1) * 16 * MT * 8 <= off_q && bytes <= 227 * 1024, "shared memory");
+    static constexpr uint32_t off_o = 0, off_ml = kFewWarps * kFewRows * HD * 4;
+    static_assert(off_ml + (kFewWarps + 1) * kFewRows * 8 <= off_q && bytes <= 227 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1)
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
     for (uint32_t i = 0; i < NS; ++i) fill();
 
     // ---- Q: rows dealt to the warps, fragments of hi and lo, score factors, masks ----
-    for (uint32_t r = warp; r < 16 * MT; r += kFewWarps) {
+    for (uint32_t r = warp; r < kFewRows; r += kFewWarps) {
         const bool mine = r < rows;
         const uint32_t tok = mine ? r / p.group : 0;
         float4 f = make_float4(0, 0, 0, 0);
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
             split_f16(f.x * sc, f.y * sc, h0, l0);
             split_f16(f.z * sc, f.w * sc, h1, l1);
             // dimensions 16 ks + 4 t ..: registers (row half) and 2 + (row half) of lane 4 g + t
-            uint32_t *dst = reinterpret_cast<uint32_t *>(smem + S::off_q + ((r / 16) * KS + lane / 4) * S::q_step) +
+            uint32_t *dst = reinterpret_cast<uint32_t *>(smem + S::off_q + lane / 4 * S::q_step) +
                             ((r & 7) * 4 + (lane & 3)) * 4 + ((r >> 3) & 1);
             dst[0] = h0, dst[2] = h1;
             dst[32 * 4] = l0, dst[32 * 4 + 2] = l1;
@@ -184,22 +184,20 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
     }
     __syncthreads();
 
-    // a lane's rows: 16 mt + g8 (i even) and 16 mt + g8 + 8
-    float cq[2 * MT], m[2 * MT], l[2 * MT];
+    // a lane's rows: g8 (i = 0) and g8 + 8
+    float cq[2], m[2], l[2];
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-        cq[i] = cqs[(i / 2) * 16 + g8 + (i & 1) * 8];
+    for (int i = 0; i < 2; ++i) {
+        cq[i] = cqs[g8 + i * 8];
         m[i] = -INFINITY;
         l[i] = 0.0f;
     }
-    const bool far = rows_far(tops[lane % (16 * MT)], p.reach);
-    float acc[MT][4 * QG][4];  // column (q, i): dimensions 32 q + 4 col + i, col 2 t4 and 2 t4 + 1
+    const bool far = rows_far(tops[lane % kFewRows], p.reach);
+    float acc[4 * QG][4];  // column (q, i): dimensions 32 q + 4 col + i, col 2 t4 and 2 t4 + 1
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int k = 0; k < 4 * QG; ++k)
 #pragma unroll
-        for (int k = 0; k < 4 * QG; ++k)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) acc[mt][k][v] = 0.0f;
+        for (int v = 0; v < 4; ++v) acc[k][v] = 0.0f;
     // places of the 16 from p0 that row r sees
     auto visible = [&](uint32_t r, uint32_t p0) -> uint32_t {
         uint32_t vis = 0xFFFFu;
@@ -222,14 +220,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
     };
     for (uint32_t c = 0; c < nc; ++c) {
         const uint32_t p0 = first_of(c), none0 = p0 + kFewUnit > places ? (0xFFFFu << (places - p0)) & 0xFFFFu : 0;
-        // ---- S: 16 MT rows x 16 places (column tiles of 8) ----
-        float s[MT][2][4];
+        // ---- S: 16 rows x 16 places (column tiles of 8) ----
+        float s[2][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                for (int v = 0; v < 4; ++v) s[mt][nt][v] = 0.0f;
+            for (int v = 0; v < 4; ++v) s[nt][v] = 0.0f;
         uint32_t sl = (2 * c) % NS;
         landed();
         const uint32_t hide = hides[c & 3], none = hide | none0;
@@ -271,16 +267,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
                     split_f16(f.x, f.y, h[nt][0], lo[nt][0]);
                     split_f16(f.z, f.w, h[nt][1], lo[nt][1]);
                 }
+                const uint4 *qf = reinterpret_cast<const uint4 *>(smem + S::off_q + ks * S::q_step) + lane;
+                const uint4 qh = qf[0], ql = qf[32];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    const uint4 *qf = reinterpret_cast<const uint4 *>(smem + S::off_q + (mt * KS + ks) * S::q_step) + lane;
-                    const uint4 qh = qf[0], ql = qf[32];
-#pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
-                        mma_f16(s[mt][nt], qh, h[nt][0], h[nt][1]);
-                        mma_f16(s[mt][nt], ql, h[nt][0], h[nt][1]);
-                        mma_f16(s[mt][nt], qh, lo[nt][0], lo[nt][1]);
-                    }
+                for (int nt = 0; nt < 2; ++nt) {
+                    mma_f16(s[nt], qh, h[nt][0], h[nt][1]);
+                    mma_f16(s[nt], ql, h[nt][0], h[nt][1]);
+                    mma_f16(s[nt], qh, lo[nt][0], lo[nt][1]);
                 }
             }
         }
@@ -296,17 +289,17 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
                 for (int v = 0; v < 2; ++v) {
                     const int own = __shfl_sync(0xffffffffu, kpe, 8 * nt + 2 * t4 + v), e = kwide ? own : ke;
 #pragma unroll
-                    for (int i = 0; i < 2 * MT; ++i) s[i / 2][nt][(i & 1) * 2 + v] = place_score(s[i / 2][nt][(i & 1) * 2 + v], cq[i], e);
+                    for (int i = 0; i < 2; ++i) s[nt][2 * i + v] = place_score(s[nt][2 * i + v], cq[i], e);
                 }
         }
-        float corr[2 * MT];
+        float corr[2];
         bool rescale = false;
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
-            float *s0 = &s[i / 2][0][(i & 1) * 2], *s1 = &s[i / 2][1][(i & 1) * 2];
+        for (int i = 0; i < 2; ++i) {
+            float *s0 = &s[0][2 * i], *s1 = &s[1][2 * i];
             const float cqk = apart ? 1.0f : score_factor(cq[i], ke);
             if (masked) {
-                const uint32_t vis = visible((i / 2) * 16 + g8 + (i & 1) * 8, p0) & ~none;
+                const uint32_t vis = visible(g8 + i * 8, p0) & ~none;
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
                     if (kbad >> (2 * t4 + v) & 1) s0[v] = NAN;
@@ -331,21 +324,16 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
         }
         if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int k = 0; k < 4 * QG; ++k)
 #pragma unroll
-                for (int k = 0; k < 4 * QG; ++k)
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) acc[mt][k][v] *= corr[2 * mt + v / 2];
+                for (int v = 0; v < 4; ++v) acc[k][v] *= corr[v / 2];
         }
-        uint4 ph[MT], pl[MT];  // P's fragments: rows g8, g8 + 8 of columns 2 t4, then of 8 + 2 t4
+        uint4 ph, pl;  // P's fragments: rows g8, g8 + 8 of columns 2 t4, then of 8 + 2 t4
         auto split_p = [&]() {
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                cut_f16(s[mt][0][0], s[mt][0][1], ph[mt].x, pl[mt].x);
-                cut_f16(s[mt][0][2], s[mt][0][3], ph[mt].y, pl[mt].y);
-                cut_f16(s[mt][1][0], s[mt][1][1], ph[mt].z, pl[mt].z);
-                cut_f16(s[mt][1][2], s[mt][1][3], ph[mt].w, pl[mt].w);
-            }
+            cut_f16(s[0][0], s[0][1], ph.x, pl.x);
+            cut_f16(s[0][2], s[0][3], ph.y, pl.y);
+            cut_f16(s[1][0], s[1][1], ph.z, pl.z);
+            cut_f16(s[1][2], s[1][3], ph.w, pl.w);
         };
         split_p();
         // ---- O: the lane's V: places 2 t4, 2 t4 + 1, 8 + 2 t4, 9 + 2 t4, dimensions 32 q + 4 g8 .. ----
@@ -382,8 +370,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
             const float sc = pow2i(-ve);
             if (__builtin_expect(vbad != 0, 0)) {  // the rows that see a place with a NaN or infinity become NaN
 #pragma unroll
-                for (int i = 0; i < 2 * MT; ++i)
-                    if ((vbad & ~none & visible((i / 2) * 16 + g8 + (i & 1) * 8, p0)) != 0) l[i] = NAN;
+                for (int i = 0; i < 2; ++i)
+                    if ((vbad & ~none & visible(g8 + i * 8, p0)) != 0) l[i] = NAN;
             }
             auto values = [&](auto &&osc) {  // osc(i): what row i's products are added with
 #pragma unroll
@@ -397,15 +385,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
                         uint32_t h0, h1, l0, l1;
                         split_f16(y[0], y[1], h0, l0);
                         split_f16(y[2], y[3], h1, l1);
+                        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma_f16(o, ph, h0, h1);
+                        mma_f16(o, pl, h0, h1);
+                        mma_f16(o, ph, l0, l1);
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma_f16(o, ph[mt], h0, h1);
-                            mma_f16(o, pl[mt], h0, h1);
-                            mma_f16(o, ph[mt], l0, l1);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) acc[mt][4 * q + v][k] = fmaf(o[k], osc(2 * mt + k / 2), acc[mt][4 * q + v][k]);
-                        }
+                        for (int k = 0; k < 4; ++k) acc[4 * q + v][k] = fmaf(o[k], osc(k / 2), acc[4 * q + v][k]);
                     }
                 }
             };
@@ -413,19 +398,19 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
                 const float vsc = pow2i(ve - (int)kRowsP);
                 values([=](int) { return vsc; });
             } else {  // P gets the places' scales relative to the row's largest weighted place
-                float rsc[2 * MT];
+                float rsc[2];
                 int pe[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) pe[k] = __shfl_sync(0xffffffffu, vpe, 2 * t4 + (k & 1) + (k >> 1) * 8);
 #pragma unroll
-                for (int i = 0; i < 2 * MT; ++i) {
+                for (int i = 0; i < 2; ++i) {
                     int em = -100;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) em = max(em, weight_exp(s[i / 2][k >> 1][(i & 1) * 2 + (k & 1)], pe[k]));
+                    for (int k = 0; k < 4; ++k) em = max(em, weight_exp(s[k >> 1][2 * i + (k & 1)], pe[k]));
                     em = max(em, __shfl_xor_sync(0xffffffffu, em, 1));
                     em = max(em, __shfl_xor_sync(0xffffffffu, em, 2));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) s[i / 2][k >> 1][(i & 1) * 2 + (k & 1)] *= pow2c(pe[k] - em);
+                    for (int k = 0; k < 4; ++k) s[k >> 1][2 * i + (k & 1)] *= pow2c(pe[k] - em);
                     rsc[i] = pow2i(em - (int)kRowsP);
                 }
                 split_p();
@@ -438,21 +423,20 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
     if (fault) raise_error(a.err, fault);
     // ---- the warps' sums, joined in warp order, where the rings were ----
     __syncthreads();
-    float *O = reinterpret_cast<float *>(smem + S::off_o) + (size_t)warp * 16 * MT * HD;
+    float *O = reinterpret_cast<float *>(smem + S::off_o) + (size_t)warp * kFewRows * HD;
     float2 *ML = reinterpret_cast<float2 *>(smem + S::off_ml);
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
+    for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        const uint32_t r = (i / 2) * 16 + g8 + (i & 1) * 8;
-        if (t4 == 0) ML[warp * 16 * MT + r] = make_float2(m[i], l[i] * pow2i(-(int)kRowsP));
+        const uint32_t r = g8 + i * 8;
+        if (t4 == 0) ML[warp * kFewRows + r] = make_float2(m[i], l[i] * pow2i(-(int)kRowsP));
 #pragma unroll
         for (int q = 0; q < QG; ++q)
 #pragma unroll
             for (int col = 0; col < 2; ++col)
                 *reinterpret_cast<float4 *>(O + r * HD + 32 * q + 4 * (2 * t4 + col)) =
-                    make_float4(acc[i / 2][4 * q][(i & 1) * 2 + col], acc[i / 2][4 * q + 1][(i & 1) * 2 + col],
-                                acc[i / 2][4 * q + 2][(i & 1) * 2 + col], acc[i / 2][4 * q + 3][(i & 1) * 2 + col]);
+                    make_float4(acc[4 * q][2 * i + col], acc[4 * q + 1][2 * i + col], acc[4 * q + 2][2 * i + col], acc[4 * q + 3][2 * i + col]);
     }
     __syncthreads();
     // A thread joins the warps' four dimensions of a row. In a cluster it leaves the result
@@ -469,21 +453,21 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
         if (d >= hd) continue;
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) M = fmaxf(M, ML[w * 16 * MT + r].x);
+        for (int w = 0; w < kFewWarps; ++w) M = fmaxf(M, ML[w * kFewRows + r].x);
         const float ref = M == -INFINITY ? 0.0f : M;
         float4 o = make_float4(0, 0, 0, 0);
         float L = 0.0f;
 #pragma unroll
         for (int w = 0; w < kFewWarps; ++w) {
-            const float2 ml = ML[w * 16 * MT + r];
+            const float2 ml = ML[w * kFewRows + r];
             const float f = ex2(ml.x - ref);
-            const float4 x = *reinterpret_cast<const float4 *>(O0 + ((size_t)w * 16 * MT + r) * HD + d);
+            const float4 x = *reinterpret_cast<const float4 *>(O0 + ((size_t)w * kFewRows + r) * HD + d);
             L = fmaf(ml.y, f, L);
             o = make_float4(fmaf(x.x, f, o.x), fmaf(x.y, f, o.y), fmaf(x.z, f, o.z), fmaf(x.w, f, o.w));
         }
         if (p.splits > 1) {
             *reinterpret_cast<float4 *>(O0 + (size_t)r * HD + d) = o;
-            if (d == 0) ML[kFewWarps * 16 * MT + r] = make_float2(M, L);
+            if (d == 0) ML[kFewWarps * kFewRows + r] = make_float2(M, L);
         } else {
             finish(r, d, L, o);
         }
@@ -501,7 +485,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 1) attn_few_kernel(const RowsP
             ml[s] = make_float2(-INFINITY, 0.0f);
             x[s] = make_float4(0, 0, 0, 0);
             if (s < p.splits) {
-                ml[s] = cluster_ld2(&ML[kFewWarps * 16 * MT + r], s);
+                ml[s] = cluster_ld2(&ML[kFewWarps * kFewRows + r], s);
                 x[s] = cluster_ld4(O0 + (size_t)r * HD + d, s);
                 M = fmaxf(M, ml[s].x);
             }
