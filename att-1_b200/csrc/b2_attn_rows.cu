@@ -69,6 +69,10 @@ template <int HD>
 struct RowsSmem {
     static constexpr uint32_t stages = 2;                           // operands of two tiles
     static constexpr uint32_t slots = HD == 128 ? 3 : 6;           // ring of f32 tiles, K and V in turn
+    // A slot's fill is waited for by parity, so every warp has to see every phase of a barrier it
+    // waits on. Where a slot is K's and V's in turn (an odd number of slots), whose warps are not
+    // the same, each has a barrier of its own there: that of fill i is i % fills.
+    static constexpr uint32_t fills = slots % 2 ? 2 * slots : slots;
     static constexpr uint32_t slot = kRowsKeys * HD * 4;
     static constexpr uint32_t half = kRowsKeys * HD * 2;           // hi or lo of an operand
     static constexpr uint32_t off_k = 0;
@@ -81,7 +85,7 @@ struct RowsSmem {
     static constexpr uint32_t off_ve = off_ke + kRowsMeta * kRowsKeys;  // [2][64] s8: of V
     static constexpr uint32_t off_rh = off_ve + 2 * kRowsKeys;      // [slots] u64: places whose page is bad
     static constexpr uint32_t off_bar = off_rh + 8 * slots;
-    static constexpr uint32_t bytes = off_bar + 8 * (2 * slots + 12) + 48;
+    static constexpr uint32_t bytes = off_bar + 8 * (fills + slots + 12) + 48;
 };
 static_assert(RowsSmem<128>::bytes <= 227 * 1024 && RowsSmem<64>::bytes <= 227 * 1024, "shared memory");
 
@@ -89,7 +93,7 @@ template <int HD, bool EXACT>
 __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsParams p)
 {
     using S = RowsSmem<HD>;
-    constexpr uint32_t NR = S::slots;
+    constexpr uint32_t NR = S::slots, NF = S::fills;
     extern __shared__ __align__(1024) uint8_t smem[];
     const b2_attn_rows_args &a = p.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -100,7 +104,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
     int8_t *kexp = reinterpret_cast<int8_t *>(smem + S::off_ke), *vexp = reinterpret_cast<int8_t *>(smem + S::off_ve);
     uint64_t *rhide = reinterpret_cast<uint64_t *>(smem + S::off_rh);
     // by parity of the tile: K and V converted, S and O computed (which frees that K and V)
-    uint64_t *r_full = reinterpret_cast<uint64_t *>(smem + S::off_bar), *r_empty = r_full + NR, *k_full = r_empty + NR,
+    uint64_t *r_full = reinterpret_cast<uint64_t *>(smem + S::off_bar), *r_empty = r_full + NF, *k_full = r_empty + NR,
              *v_full = k_full + 2, *s_full = v_full + 2, *o_full = s_full + 2, *s_empty = o_full + 2, *p_full = s_empty + 1,
              *q_full = p_full + 1, *done = q_full + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1), *met = tmem_slot + 2;  // [4][2]: the halves' meetings
@@ -123,10 +127,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
     const uint32_t nsoft = 2 * ((live + 31) / 32);  // softmax warps with rows: two per quarter of the rows
 
     if (threadIdx.x == 0) {
-        for (uint32_t i = 0; i < NR; ++i) {
-            mbar_init(&r_full[i], 1);
-            mbar_init(&r_empty[i], kRowsKeys / kRowsUnit);
-        }
+        for (uint32_t i = 0; i < NF; ++i) mbar_init(&r_full[i], 1);
+        for (uint32_t i = 0; i < NR; ++i) mbar_init(&r_empty[i], kRowsKeys / kRowsUnit);
         for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(&k_full[i], kRowsKeys / kRowsUnit);
             mbar_init(&v_full[i], kRowsKeys / kRowsUnit);
@@ -186,9 +188,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                     const uint32_t i = 2 * j + op, sl = i % NR;
                     if (i >= NR) ok = warp_wait(&r_empty[sl], i / NR - 1, a.err);
                     if (!ok) break;
+                    uint64_t *full = &r_full[i % NF];
                     if (lane == 0) {
                         rhide[sl] = (uint64_t)bad[1] << 32 | bad[0];
-                        mbar_arrive_expect_tx(&r_full[sl], bytes);
+                        mbar_arrive_expect_tx(full, bytes);
                     }
                     __syncwarp();
                     const float *pool = op == 0 ? a.kv.k_pool : a.kv.v_pool;
@@ -196,12 +199,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
                     for (uint32_t h = 0; h < 2; ++h)
                         if (run[h] != 0)
                             bulk_g2s_stream(smem + S::off_r + sl * S::slot + (lane + 32 * h) * rowb, pool + row[h], run[h] * rowb,
-                                            &r_full[sl], pol);
+                                            full, pol);
                     filled = i + 1;
                 }
             }
             // no copy is in flight when the CTA ends, not even after a wait that gave up
-            for (uint32_t i = filled > NR ? filled - NR : 0; i < filled; ++i) warp_wait(&r_full[i % NR], i / NR, a.err);
+            for (uint32_t i = filled > NR ? filled - NR : 0; i < filled; ++i) warp_wait(&r_full[i % NF], i / NF, a.err);
             if (fault) raise_error(a.err, fault);
         } else if (warp == kRowsMmaWarp) {
             // ---- MMA issue ----
@@ -251,16 +254,16 @@ __global__ void __launch_bounds__(kRowsThreads, 1) attn_rows_kernel(const RowsPa
     } else if (warp >= (uint32_t)kRowsSoftWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRowsConvRegs));
         // ---- ring tiles into operands ----
-        // Every warp takes part in every tile's K, or in every tile's V, so none can be two
-        // phases of a barrier away from the others. K and V differ in how a lane picks its
-        // values; the conversion of its HD / 32 chunks of eight (16 bytes of hi, 16 of lo) is
-        // one piece of code for both: the roles of this kernel run different code side by
-        // side, and instruction fetch is what they run out of first.
+        // Every warp takes part in every tile's K, or in every tile's V, so (with r_full apart for
+        // the two) none can be two phases of a barrier away from the others. K and V differ in
+        // how a lane picks its values; the conversion of its HD / 32 chunks of eight (16 bytes of
+        // hi, 16 of lo) is one piece of code for both: the roles of this kernel run different
+        // code side by side, and instruction fetch is what they run out of first.
         const bool is_v = warp >= (uint32_t)kRowsSoftWarps + 4;
         for (uint32_t j = 0; j < nt; ++j) {
             const uint32_t i = 2 * j + is_v, sl = i % NR;
             const uint32_t st = j & 1;
-            if (!warp_wait(&r_full[sl], i / NR, a.err)) break;
+            if (!warp_wait(&r_full[i % NF], i / NF, a.err)) break;
             if (j >= 2 && !warp_wait((is_v ? o_full : s_full) + st, j / 2 - 1, a.err)) break;
             const uint64_t hide = rhide[sl];
 #pragma unroll 1

@@ -215,6 +215,35 @@ def test_attn_scores_in_range_of_operands_far_from_one(b2, torch, h, hkv, hd, ne
     assert np.abs(got[rows] - ref[rows]).max() <= 2.0 ** -19 * np.nanmax(np.abs(s.v))
 
 
+@pytest.mark.parametrize("h,hkv,hd,new", [(8, 2, 128, 24), (10, 2, 80, 20), (8, 2, 64, 24)])
+def test_attn_pages_far_apart(b2, torch, h, hkv, hd, new):
+    """Every page 64 MB from the next, so the copies of K and V come in at times of their own, in an order other than they were
+    asked for; the same bits each time."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("not enough device memory free")
+    page = 16
+    s = Scene(torch, h, hkv, hd, page, [1500, 700], [new, new], seed=25)
+    a = s.args(b2)
+    stride = (64 << 20) // (hkv * page * hd * 4)
+    used = np.unique(s.table[s.table >= 0])
+    k, v = (torch.empty(stride * (s.pool_pages + 1), hkv, page, hd, device="cuda") for _ in range(2))
+    at = dev(torch, used, np.int64)
+    k[at * stride], v[at * stride] = s.d["k"][at], s.d["v"][at]
+    far = dev(torch, np.where(s.table >= 0, s.table * stride, s.table), np.int32)
+    a.kv.k_pool, a.kv.v_pool, a.kv.page_table, a.pool_pages = p(k), p(v), p(far), k.shape[0]
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    ref, first = s.reference(), None
+    for _ in range(12):
+        flush.zero_()
+        s.d["out"].zero_()
+        assert b2.lib().b2_attn_rows(a, None) == 0
+        torch.cuda.synchronize()
+        got = s.d["out"].cpu().numpy()[:s.rows, :h * hd].reshape(s.rows, h, hd)
+        assert int(s.d["err"].item()) == 0 and np.abs(got - ref).max() <= ATTN_TOL * 5
+        assert first is None or (got == first).all()
+        first = got
+
+
 # ---- b2_kv_plan, b2_rows_append -----------------------------------------------------------------------------
 
 
