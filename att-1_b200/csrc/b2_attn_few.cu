@@ -6,10 +6,11 @@
 // With few rows the work is the stream of K and V, so the kernel is built around it:
 // CTA (split, KV head, item) takes a contiguous range of the places, its eight warps
 // 16 places each in turn. A warp owns a ring of shared-memory slots that it fills with
-// cp.async (an SM works bulk copies off one after the other, about 0.45 us each, so
-// eight warps' small ones would queue for 7 us) and waits for nobody: it reads a slot
-// straight into mma.sync fragments (m16n8k16), converting in registers, so K and
-// V cross shared memory once and no warp synchronises with another before the end.
+// cp.async (every lane copies its own pieces, of places on any page; a bulk copy per run
+// of places would take the thread that issues it some 300 cycles each) and waits for
+// nobody: it reads a slot straight into mma.sync fragments (m16n8k16), converting in
+// registers, so K and V cross shared memory once and no warp synchronises with another
+// before the end.
 //   S = Q K^T: the fragment of Q comes from shared memory (prepared once); a lane's four
 //   K values of a 16-dimension step are consecutive (both operands take the
 //   dimensions of a step in the order 4 t, 4 t + 1 | 4 t + 2, 4 t + 3).

@@ -620,22 +620,26 @@ constexpr size_t kLaidBytes = (size_t)512 << 20;
 // places go to attn_few_kernel, which converts K and V in registers and multiplies with
 // mma.sync: no tensor-memory set-up, no roles to synchronise, no 128-row products for a
 // handful of rows, no second kernel. Against attn_rows_kernel, one token of the 8B shape
-// (4 rows) at context 1000 9.9 us and 15.1, 1900 13.4 and 18.1, 4000 22.9 and 23.0; 8
-// sequences of it 24.7 and 25.6, 39.6 and 39.0, 72.0 and 71.9. (For 32 rows it lost: 8
-// sequences of 8 tokens at context 1000 35 and 28.)
+// (4 rows) at context 1000 9.8 us and 14.8, 1900 13.5 and 17.7, 4000 23.9 and 23.0; 8
+// sequences of it 25.0 and 25.2, 40.9 and 39.0, 77.6 and 71.1. (A form for 32 rows took 8
+// tokens at context 1000 in 15.7, where attn_rows_kernel takes 16.5, but 8 sequences of
+// that in 35, against 28.)
 //
 // From kLaidBlocks blocks of 128 rows on, K and V are laid out as operands once for all of
 // them (b2_attn_laid.cu). 2000 cached places, laid out and each block for itself: 8B shape,
-// 8 sequences of 128 rows (4 blocks) 122 us and 138, 512 rows (16 blocks) 67 and 94; 8
-// sequences of 64 (2 blocks) 82 and 79.5; 9 heads of 64, 8 sequences of 64 rows (2 blocks)
-// 35.7 and 30.7. That takes scratch of the size of the batch's K and V, and is left out
+// 8 sequences of 128 rows (4 blocks) 123 us and 143, 512 rows (16 blocks) 67 and 97; 8
+// sequences of 64 (2 blocks) 79.1 and 80.7; 9 heads of 64, 8 sequences of 64 rows (2 blocks)
+// 33.9 and 31.0. That takes scratch of the size of the batch's K and V, and is left out
 // where it would be more than kLaidBytes.
 //
 // The splits take the least modelled time, in quarters of a tile's: what a CTA costs besides
 // its tiles (launch, q, the pipeline's ends) and what joining costs, by a kernel also one
-// per split. Measured (8B shape, attn_rows_kernel): 8 tokens at context 1000 8 splits 17.8
-// us, 16 splits 21.2, 4 19.0; one KV head of the 70B shape, 8 sequences of 30000 18 splits
-// 82.8 us, 12 97.9, 24 98.2.
+// per split. Measured (attn_rows_kernel): 8B shape, 8 tokens at context 1000 8 splits 16.5
+// us, 16 splits 17.8, 4 18.6; one KV head of the 70B shape, 8 sequences to 30000 18 splits
+// 78 us, 12 97, 24 91. Items of different lengths have the same number of splits: evener
+// shares were worth little where a call is long enough for the power cap (8B shape, 16
+// trees of 32, contexts 4000 to 8000: 1 to 4 splits 288 to 290 us, at 990 W and 1770 to
+// 1687 MHz; 261 to 252 from rest).
 static void attn_rows_plan(const b2_attn_rows_args *a, RowsParams &p, bool &few)
 {
     p.group = a->n_heads / a->n_kv_heads;
