@@ -134,7 +134,7 @@ __device__ __forceinline__ void stage_q(const RowsParams &p, uint32_t w, uint32_
             const uint32_t r = b + 8 * i, m_row = first + r;
             f[i] = make_float4(0, 0, 0, 0);
             if (r < live && 4 * lane < hd)
-                f[i] = reinterpret_cast<const float4 *>(a.q + (size_t)(r0 + m_row / p.group) * a.q_stride + (size_t)(kvh * p.group + m_row % p.group) * hd)[lane];
+                f[i] = __ldcg(reinterpret_cast<const float4 *>(a.q + (size_t)(r0 + m_row / p.group) * a.q_stride + (size_t)(kvh * p.group + m_row % p.group) * hd) + lane);
         }
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; ++i) {
@@ -200,10 +200,12 @@ __global__ void __launch_bounds__(kLaidThreads, 1) attn_laid_kernel(const RowsPa
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 2);
 
     // Launched while attn_rows_lay_kernel still runs: what came before that has completed, and
-    // only the copies read what it writes.
+    // only the copies read what it writes. The lengths, q and the masks are read without this
+    // kernel's own wait, so from L2: nothing says that an SM's L1 no longer holds what the same
+    // buffers had in the layer before.
     pdl_launch_dependents();
     uint32_t r0, n, ctx;
-    if (!rows_item(a, item, r0, n, ctx)) {
+    if (!rows_fit(a, __ldcg(a.row_start + item), __ldcg(a.row_start + item + 1), __ldcg(a.ctx_len + item), r0, n, ctx)) {
         if (threadIdx.x == 0 && split == 0 && blockIdx.y == 0) raise_error(a.err, B2_ERR_POSITION);
         pdl_wait();
         return;
@@ -437,7 +439,7 @@ __global__ void __launch_bounds__(kLaidThreads, 1) attn_laid_kernel(const RowsPa
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
-            const uint64_t mask = mine && a.tree != nullptr ? a.tree[r0 + tok] : 0;
+            const uint64_t mask = mine && a.tree != nullptr ? __ldcg(reinterpret_cast<const unsigned long long *>(a.tree) + r0 + tok) : 0;
             float m = -INFINITY, l = 0.0f;
             bool ok = true;
             // One tile; those with units of different scale, marked places or scores past 2^23 have

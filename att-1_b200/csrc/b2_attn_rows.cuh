@@ -26,9 +26,8 @@ struct RowsParams {
 };
 
 // The rows of an item, or false for lengths that do not fit.
-__device__ __forceinline__ bool rows_item(const b2_attn_rows_args &a, uint32_t item, uint32_t &r0, uint32_t &n, uint32_t &ctx)
+__device__ __forceinline__ bool rows_fit(const b2_attn_rows_args &a, int32_t s, int32_t e, int32_t c, uint32_t &r0, uint32_t &n, uint32_t &ctx)
 {
-    const int32_t s = a.row_start[item], e = a.row_start[item + 1], c = a.ctx_len[item];
     if (s < 0 || e < s || (uint32_t)e > a.rows || (uint32_t)(e - s) > a.max_rows || c < 0 || (uint32_t)c > a.max_ctx ||
         (uint32_t)(e - s) > a.max_ctx - (uint32_t)c || (a.tree != nullptr && e - s > B2_MAX_TREE))
         return false;
@@ -36,6 +35,10 @@ __device__ __forceinline__ bool rows_item(const b2_attn_rows_args &a, uint32_t i
     n = (uint32_t)(e - s);
     ctx = (uint32_t)c;
     return true;
+}
+__device__ __forceinline__ bool rows_item(const b2_attn_rows_args &a, uint32_t item, uint32_t &r0, uint32_t &n, uint32_t &ctx)
+{
+    return rows_fit(a, a.row_start[item], a.row_start[item + 1], a.ctx_len[item], r0, n, ctx);
 }
 
 // Places a block of rows can see, and the units [t0, t1) of split s.

@@ -244,6 +244,57 @@ def test_attn_pages_far_apart(b2, torch, h, hkv, hd, new):
         first = got
 
 
+@pytest.mark.parametrize("h,hkv,hd,new", [(8, 1, 128, [130, 64]), (8, 2, 64, [200, 40]), (8, 2, 128, [20, 31]), (4, 2, 64, [6, 8])])
+def test_attn_layers_share_q_and_scratch(b2, torch, h, hkv, hd, new):
+    """Append and attention of eight layers through one q buffer and one scratch, each kernel launched while the one before still
+    runs, captured and replayed: the bits of each layer by itself."""
+    L, layers, page, batch = b2.lib(), 8, 16, len(new)
+    rng = np.random.default_rng(hd + h)
+    ctx, rows = [150, 37], sum(new)
+    start = np.concatenate([[0], np.cumsum(new)])
+    pps = max(-(-(c + n) // page) for c, n in zip(ctx, new))
+    pool = batch * pps
+    tab = rng.permutation(pool).reshape(batch, pps)
+    slot = [int(tab[b, (ctx[b] + i) // page]) * page + (ctx[b] + i) % page for b in range(batch) for i in range(new[b])]
+    d = dict(start=dev(torch, start, np.int32), ctx=dev(torch, ctx, np.int32), table=dev(torch, tab, np.int32), slot=dev(torch, slot, np.int32))
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(7)
+    y = torch.randn(layers, rows, (h + 2 * hkv) * hd, generator=g, device="cuda")
+    k, v = (torch.randn(layers, pool, hkv, page, hd, generator=g, device="cuda") for _ in range(2))
+    q, o = torch.zeros(rows, h * hd, device="cuda"), torch.zeros(layers, rows, h * hd, device="cuda")
+    scratch = None
+
+    def layer(i, stream, pdl):
+        nonlocal scratch
+        kv = b2.KVLayout(p(k[i]), p(v[i]), p(d["table"]), page, pps, hkv, hd)
+        b2.check("append", L.b2_rows_append(b2.RowsAppendArgs(m=rows, y=p(y[i]), y_stride=y.shape[2], q_rows=h * hd, q=p(q), q_stride=h * hd,
+                                                              slots=p(d["slot"]), kv=kv, pool_pages=pool, err=p(err), pdl=pdl), stream))
+        a = b2.AttnRowsArgs(batch=batch, n_heads=h, n_kv_heads=hkv, head_dim=hd, max_rows=max(new), rows=rows, q=p(q), q_stride=h * hd, kv=kv,
+                            pool_pages=pool, row_start=p(d["start"]), ctx_len=p(d["ctx"]), max_ctx=pps * page, ctx=p(o[i]),
+                            ctx_stride=h * hd, err=p(err), pdl=pdl)
+        need = L.b2_attn_rows_scratch_bytes(a)
+        if scratch is None:
+            scratch = torch.empty(need + 16, dtype=torch.uint8, device="cuda")
+        a.scratch, a.scratch_bytes = p(scratch), need
+        b2.check("attn", L.b2_attn_rows(a, stream))
+
+    for i in range(layers):
+        layer(i, None, 0)
+        torch.cuda.synchronize()
+    want = o.clone()
+    st = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        for i in range(layers):
+            layer(i, torch.cuda.current_stream().cuda_stream, 1)
+    for _ in range(20):
+        o.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(err.item()) == 0 and (o == want).all()
+
+
 # ---- b2_kv_plan, b2_rows_append -----------------------------------------------------------------------------
 
 
