@@ -19,8 +19,8 @@
 // An MMA of 128 rows and K = 16 costs 64 cycles with N = 128 and hardly less with fewer, so
 // S is taken of pairs of tiles. S of a pair, two P, q and O fill the 512 columns.
 //
-// 8B shape: a chunk of 512 at context 2500 75 us with the conversion (8 us), 308 TFLOP/s
-// of f32 products (three f16 products each); 2000 rows at context 6000 616 us. Each block
+// 8B shape: a chunk of 512 at context 2500 77 us with the conversion (8 us), 300 TFLOP/s
+// of f32 products (three f16 products each); 2000 rows at context 6000 634 us. Each block
 // converting for itself: 110 and 992 us. A tile takes 2500 cycles, its MMAs 1580: O of a tile
 // (800), its reading out (600) and the hand-overs between the roles (200 to 300 each) follow
 // one another, because tensor memory has no room for a second O.
